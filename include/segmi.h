@@ -505,6 +505,69 @@ int segmi_sgd_step(const segmi_sgd_chunk* table, int nchunks, const float* lr_ho
 int segmi_sgd_hyper_floats(void);
 int segmi_sgd_step_dev(const segmi_sgd_chunk* table, int nchunks, const float* hyper_dev, segmi_stream_t stream);
 
+/* ------------------------------------------------------------------ matrix optimizer (Muon) and AdamW
+ * Optimizers of large language models beside SGD: the reference resolves `optimizer.type` by name in torch.optim
+ * (base/base_trainer.py:57) and has none of its own.
+ *
+ * Orthogonalisation by Newton-Schulz products: X = G / max(|G|_F, eps), then `steps` times
+ *     X <- (a I + b X X^T + c (X X^T)^2) X        (on the shorter side of G; a, b, c = coefficients_host[0..2])
+ * dst = X in G's type.  Element (r, c) of a matrix lies at r * rs + c * cs (elements; any strides, also 0 in src).  fp32 accuracy
+ * (products of fp16 pairs, fp32 accumulators); NaN or infinity anywhere in a matrix makes all of its result NaN.  `dst` must not
+ * overlap any `src`.  The descriptor arrays are HOST memory, read before the call returns; the workspace is aligned to 256 bytes. */
+#define SEGMI_NS_MAX_STEPS 32
+typedef struct segmi_ns_matrix {
+    const void* src;
+    void* dst;
+    long src_rs, src_cs, dst_rs, dst_cs;
+    int rows, cols;
+    int dtype; /* 0 fp32, 1 bf16: src and dst */
+    int reserved;
+} segmi_ns_matrix;
+/* bytes; 0 = a shape is not supported (a side < 1, or 4 GiB and more of fp32 values after padding both sides to 64) */
+size_t segmi_ns_workspace(const segmi_ns_matrix* mats_host, int count);
+/* 1: the iteration's singular values stay below 4096 for these coefficients (and above 1e-6 at its upper end); the calls below
+ * return SEGMI_ERR_BADARG otherwise */
+int segmi_ns_coefficients_ok(const double* coefficients_host, int steps);
+int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const double* coefficients_host, int steps, double eps,
+                           void* workspace, size_t workspace_bytes, segmi_stream_t stream);
+/* One Muon step over a set of matrices, each dense rows x cols in memory:
+ *     momentum = mu momentum + grad;   u = grad + mu momentum (nesterov) or momentum
+ *     param = (1 - lr wd) param - lr factor orthogonalize(u)
+ * lr, wd, mu per group (ngroups <= 8): host arrays, or, with hyper_dev, device memory in segmi_sgd_step_dev's layout (then the host
+ * arrays are not read). */
+typedef struct segmi_muon_matrix {
+    float* param;
+    const float* grad;
+    float* momentum;
+    int rows, cols;
+    float factor;
+    int group;
+} segmi_muon_matrix;
+size_t segmi_muon_workspace(const segmi_muon_matrix* mats_host, int count);
+int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* lr_host, const float* weight_decay_host,
+                    const float* momentum_host, int ngroups, const float* hyper_dev, int nesterov, const double* coefficients_host, int steps,
+                    double eps, void* workspace, size_t workspace_bytes, segmi_stream_t stream);
+/* AdamW (decoupled weight decay) over a set of tensors, t = the step's number counted from 1:
+ *     exp_avg = b1 exp_avg + (1 - b1) grad;   exp_avg_sq = b2 exp_avg_sq + (1 - b2) grad^2
+ *     param = (1 - lr wd) param - lr / (1 - b1^t) exp_avg / (sqrt(exp_avg_sq / (1 - b2^t)) + eps)
+ * The descriptors and the per-group hyper-parameters (SEGMI_ADAMW_HYPER doubles per group: lr, wd, b1, b2, eps;
+ * ngroups <= 8) are HOST memory read before the call returns.  `step` is t.  For a step captured into a graph pass hyper_dev (the
+ * same numbers in device memory), a device float `step_dev` per tensor, which the call advances, and a workspace of 8 bytes per tensor. */
+#define SEGMI_ADAMW_HYPER 5
+typedef struct segmi_adamw_tensor {
+    float* param;
+    const float* grad;
+    float* exp_avg;
+    float* exp_avg_sq;
+    float* step_dev;
+    double step;
+    long count;
+    int group;
+    int reserved;
+} segmi_adamw_tensor;
+int segmi_adamw_step(const segmi_adamw_tensor* tensors_host, int count, const double* hyper_host, int ngroups, const double* hyper_dev,
+                     void* workspace, size_t workspace_bytes, segmi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

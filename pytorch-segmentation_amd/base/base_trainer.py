@@ -83,10 +83,10 @@ class BaseTrainer:
         else:
             trainable_params = [p for p in self.model.parameters() if p.requires_grad]
         # same by-name resolution as the reference (`getattr(torch.optim, type)`); optimizers that exist as fused libsegmi
-        # kernels (SGD) are taken from segmi.optim — identical update rule and state layout
+        # kernels (SGD; Muon, FusedAdamW) are taken from segmi.optim — identical update rule and state layout
         otype = config["optimizer"]["type"]
         oargs = config["optimizer"]["args"]
-        fused = hasattr(segmi_optim, otype) and not oargs.get("nesterov") and not oargs.get("dampening")
+        fused = otype in ("Muon", "FusedAdamW") or (otype == "SGD" and not oargs.get("nesterov") and not oargs.get("dampening"))
         self.optimizer = get_instance(segmi_optim if fused else torch.optim, "optimizer", config, trainable_params)
         # data parallel + fused SGD: the update of a gradient bucket is launched right after ITS all-reduce (segmi.distributed)
         self.bucket_step = bool(self.model.reducer.collective and fused and self.model.attach_optimizer(self.optimizer))

@@ -20,7 +20,9 @@ LIB = os.path.join(OUT_DIR, "libsegmi.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
-FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Wno-unused-value"]
+# no packed fp32 arithmetic (v_pk_add/mul/fma_f32) in any kernel: some of its forms have given wrong results on this hardware now and then
+FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Wno-unused-value",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-file additions: no compiler-formed packed-fp32 arithmetic (v_pk_mul/fma/add_f32) in the HBM-bound kernels.  The SLP-packed
 # form of bilinear_fwd_kernel returns wrong high halves while a bf16x3 convolution kernel of ANOTHER process shares the GPU
 # (tools/probes/pk_two_process.py reproduces it with exactly these two kernels: 32 % of the launches wrong against an fp64 reference,

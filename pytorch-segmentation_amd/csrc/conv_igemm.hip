@@ -19,6 +19,7 @@
 // ds_read_b128 fragment reads are bank-conflict free (MI355X_MICROARCH.md, LDS table).
 #include <type_traits>
 #include "segmi_common.h"
+#include "lds_dma.h"
 #include "conv_internal.h"
 #include <cstdio>
 #include <cstdlib>
@@ -250,28 +251,9 @@ __global__ __launch_bounds__(256) void conv_gather_kernel(GatherParams p) {
 // builtin it does, serialising load latency and MFMA work).  We count them ourselves: one
 // `s_waitcnt vmcnt(0)` + barrier at the end of each stage.  M0 (LDS destination base) is written in
 // the same statement that consumes it.
-typedef __attribute__((address_space(3))) void lds_void;
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ i32x4 make_rsrc(const void* base, unsigned bytes) {
-    const unsigned long long a = (unsigned long long)base;
-    i32x4 r;
-    r.x = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
-    r.y = __builtin_amdgcn_readfirstlane((int)((unsigned)(a >> 32) & 0xFFFFu));   // stride 0, no swizzle
-    r.z = __builtin_amdgcn_readfirstlane((int)bytes);                              // num_records (bytes)
-    r.w = 0x00020000;                                                              // raw buffer, 32-bit data format
-    return r;
-}
-__device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(unsigned long long)(lds_void*)p; }
 __device__ __forceinline__ void dma16(const i32x4& rsrc, unsigned voffset, unsigned lds_dst) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                  :: "v"(voffset), "s"(rsrc), "s"(lds_dst) : "memory");
-}
-
-// the same with a scalar byte offset on top of the lane's (soffset field of the instruction)
-__device__ __forceinline__ void dma16s(const i32x4& rsrc, unsigned voffset, unsigned soffset, unsigned lds_dst) {
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
-                 :: "v"(voffset), "s"(rsrc), "s"(soffset), "s"(lds_dst) : "memory");
 }
 
 // FAST (R*S <= 32 taps, fprop or unit-stride dgrad): the source pixel of tap (r,s) is affine in the tap, so each DMA row

@@ -1,0 +1,949 @@
+// Orthogonalisation of matrices by Newton-Schulz products, and the Muon step around it.
+//
+// Mathematics.  X_0 = G / max(|G|_F, eps), the shorter side m as rows, the longer n as columns.  A step of the quintic iteration is
+//     A = X X^T,   Q = a I + b A + c A^2,   X <- Q X,
+// which takes every singular value s to p(s) = a s + b s^3 + c s^5.  Steps are taken on the Gram side: all of these m x m matrices are
+// polynomials of A, so X_L = (Q_{L-1} ... Q_0) X_0 with A_{k+1} = Q_k A_k Q_k, and a segment of L steps reads the large matrix twice
+// (its Gram product and the product with P = Q_{L-1} ... Q_0) instead of 2 L times.  Rounding in A_k acts on the SQUARES of
+// the singular values and is amplified by a^2 a step, so X is formed and its Gram matrix taken anew after segments of 2 and 1 steps.
+// Median distance from 64-bit results relative to the fp32 iteration's (64 x 128 noise with strong directions / 256 x 512 low rank):
+// five steps as 2 + 1 + 2: 1.06 / 1.5, one by one: 1.05 / 2.3, 1 + 2 + 2: 2.3 / 2.1, 3 + 2: 6.1 / 1.2.  Of these 2 + 1 + 2 needs
+// 9 m^2 n + 11 m^3 operations, one by one 15 m^2 n + 5 m^3 (both with symmetric products halved): the same for square matrices, fewer for
+// all others.
+//
+// Arithmetic.  Every matrix is held as hi + lo, two fp16 numbers of one value scaled by a power of two (22 - 23 significant bits; fp32
+// has 24), and a product is hi hi + hi lo + lo hi on v_mfma_f32_32x32x16_f16 with fp32 accumulators.  The dropped lo lo term and the
+// split are 2^-22 relative, and the same measurement puts the whole iteration at the distance of the fp32 one, at a third
+// of the fp16 rate = 5 times the fp32 matrix rate.  fp16's range is no obstacle here: the iterates' singular values are bounded by
+// intervals that follow from the coefficients (`Bounds` below), so each matrix gets the scale that puts its bound below 2^15; what is
+// lost below fp16's subnormal step is 2^-25 / 2^15 = 2^-40 of the largest possible entry.
+//
+// Symmetric products compute the tiles on and below the diagonal and store each twice.
+//
+// Layout.  A matrix row is a run of 128-byte lines; a line holds 32 consecutive values as 32 fp16 hi followed by 32 fp16 lo: one
+// line is one K step of a row, one DMA row of LDS, and one full HBM line.  Both dimensions are padded to 64 with zeros, so no
+// kernel but the first and the last knows a border.
+#include "segmi_common.h"
+#include "lds_dma.h"
+#include <cmath>
+#include <cstring>
+
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int BATCH = 48;            // matrices per launch: their descriptors travel as kernel arguments (< 4 KiB)
+constexpr int MAX_GROUPS = 8;
+constexpr unsigned LINE = 128;
+
+enum Buf { X = 0, T0, T1, A, Q, W, P0, P1 };
+
+// one matrix as the products see it: m <= n, both unpadded; its buffers start `base` * 256 bytes into the workspace
+struct Item {
+    unsigned first;                  // first workgroup of the launch that works on it
+    int m, n;
+    unsigned base;
+};
+struct Batch {
+    char* ws;
+    int count;
+    Item item[BATCH];
+};
+
+__host__ __device__ inline unsigned pad64(unsigned v) { return (v + 63u) & ~63u; }
+__host__ __device__ inline size_t big_bytes(int m, int n) { return (size_t)pad64(m) * pad64(n) * 4; }
+__host__ __device__ inline size_t square_bytes(int m) { return (size_t)pad64(m) * pad64(m) * 4; }
+__host__ __device__ inline size_t buffer_offset(int buf, int m, int n) {
+    return buf < A ? (size_t)buf * big_bytes(m, n) : 3 * big_bytes(m, n) + (size_t)(buf - A) * square_bytes(m);
+}
+
+// lane l looks at item l: one load and one ballot instead of a search
+template <typename B>
+__device__ __forceinline__ int find_item(const B& b, unsigned wg) {
+    const int lane = threadIdx.x & 63;
+    const unsigned first = lane < b.count ? b.item[lane].first : 0xFFFFFFFFu;
+    return __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(first <= wg)) - 1);
+}
+
+__device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
+    hi = (_Float16)v;
+    lo = (_Float16)(v - (float)hi);
+}
+// values k .. k+3 (k % 4 == 0) of a row
+__device__ __forceinline__ void store4(char* buf, unsigned lines, unsigned row, unsigned k, const float* v) {
+    f16x4 hi, lo;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        _Float16 h, l;
+        split(v[x], h, l);
+        hi[x] = h;
+        lo[x] = l;
+    }
+    char* p = buf + ((size_t)row * lines + (k >> 5)) * LINE + (k & 31) * 2;
+    *reinterpret_cast<f16x4*>(p) = hi;
+    *reinterpret_cast<f16x4*>(p + 64) = lo;
+}
+__device__ __forceinline__ void store1(char* buf, unsigned lines, unsigned row, unsigned k, float v) {
+    _Float16 h, l;
+    split(v, h, l);
+    char* p = buf + ((size_t)row * lines + (k >> 5)) * LINE + (k & 31) * 2;
+    *reinterpret_cast<_Float16*>(p) = h;
+    *reinterpret_cast<_Float16*>(p + 64) = l;
+}
+__device__ __forceinline__ void load4(const char* buf, unsigned lines, unsigned row, unsigned k, float* v) {
+    const char* p = buf + ((size_t)row * lines + (k >> 5)) * LINE + (k & 31) * 2;
+    const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + 64);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[x] = (float)hi[x] + (float)lo[x];
+}
+
+// ------------------------------------------------------------------------------------------------ reading the updates
+// An update is seen as outer x inner with the inner dimension the contiguous one where there is one.
+struct Source {
+    unsigned first;                  // workgroup of the current launch
+    unsigned base;                   // as in Item
+    const void* src;                 // MUON: the gradient
+    float* mom;                      // MUON: the momentum buffer (same order)
+    long so, si;                     // strides in elements
+    int outer, inner;
+    unsigned part, parts;            // its partial sums of squares
+    int dtype;                       // 0 fp32, 1 bf16
+    int inner_is_n;                  // 1: the inner dimension is the longer side
+    int group;
+};
+struct SourceBatch {
+    char* ws;
+    double* partial;
+    double eps;
+    float scale;                     // of X_0
+    int count;
+    int nesterov;
+    Source item[BATCH];
+};
+struct Hyper {
+    float lr[MAX_GROUPS], wd[MAX_GROUPS], mom[MAX_GROUPS];
+};
+
+__device__ __forceinline__ float bf16_to_f32(unsigned short u) { return __uint_as_float((unsigned)u << 16); }
+__device__ __forceinline__ unsigned short f32_to_bf16(float f) {
+    const unsigned u = __float_as_uint(f);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (unsigned short)((u >> 16) | 0x40u);        // NaN stays NaN
+    return (unsigned short)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);                       // round to nearest, ties to even
+}
+
+__device__ __forceinline__ float source_at(const Source& s, long off) {
+    return s.dtype ? bf16_to_f32(static_cast<const unsigned short*>(s.src)[off]) : static_cast<const float*>(s.src)[off];
+}
+
+// Sum of squares of every update in fp64 (a gradient of 1e-25 or 1e25 must not vanish or overflow), one partial per 64 x 256
+// elements, summed later in a fixed order.  MUON also advances the momentum buffer: mom = mu mom + g.
+// HBM-bound: 4 B (MUON 12 B) per element.
+template <bool MUON>
+__global__ __launch_bounds__(256) void ns_sum_squares(SourceBatch b, Hyper h, const Hyper* __restrict__ hd) {
+    const int it = find_item(b, blockIdx.x);
+    const Source& s = b.item[it];
+    const unsigned unit = blockIdx.x - s.first;
+    const unsigned across = (unsigned)(s.inner + 255) / 256;
+    const long o0 = (long)(unit / across) * 64, i0 = (long)(unit % across) * 256;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const float mu = MUON ? (hd ? hd->mom[s.group] : h.mom[s.group]) : 0.f;
+    const bool nest = MUON && b.nesterov;
+    double sum = 0.0;
+    const bool vec = s.dtype == 0 && s.si == 1 && (s.so & 3) == 0 && (s.inner & 3) == 0 && ((size_t)s.src & 15) == 0 && ((size_t)s.mom & 15) == 0;
+    for (int r = wave; r < 64; r += 4) {
+        const long o = o0 + r;
+        if (o >= s.outer) break;
+        if (vec) {
+            const long i = i0 + lane * 4;
+            if (i < s.inner) {
+                const long off = o * s.so + i;
+                const float4 gv = ld4(static_cast<const float*>(s.src) + off);
+                float g[4] = {gv.x, gv.y, gv.z, gv.w};
+                if (MUON) {
+                    const float4 mv = ld4(s.mom + off);
+                    float m[4] = {mv.x, mv.y, mv.z, mv.w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        m[x] = fmaf(mu, m[x], g[x]);
+                        g[x] = nest ? fmaf(mu, m[x], g[x]) : m[x];
+                    }
+                    st4(s.mom + off, make_float4(m[0], m[1], m[2], m[3]));
+                }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) sum = fma((double)g[x], (double)g[x], sum);
+            }
+        } else {
+            for (int x = 0; x < 4; ++x) {
+                const long i = i0 + x * 64 + lane;
+                if (i < s.inner) {
+                    const long off = o * s.so + i * s.si;
+                    float g = source_at(s, off);
+                    if (MUON) {
+                        const float m = fmaf(mu, s.mom[off], g);
+                        s.mom[off] = m;
+                        g = nest ? fmaf(mu, m, g) : m;
+                    }
+                    sum = fma((double)g, (double)g, sum);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    __shared__ double red[4];
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) b.partial[s.part + unit] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// X_0 = u / max(|u|, eps), scaled and split, in both orders (rows along n for the Gram product, rows along m for the
+// product with P), zeros in the padding; 64 x 64 elements a workgroup, turned round in LDS.
+// HBM-bound: reads 4 B (MUON 8 B), writes 8 B per element.
+template <bool MUON>
+__global__ __launch_bounds__(256) void ns_normalise(SourceBatch b, Hyper h, const Hyper* __restrict__ hd) {
+    const int it = find_item(b, blockIdx.x);
+    const Source& s = b.item[it];
+    const unsigned tile = blockIdx.x - s.first;
+    const int tid = threadIdx.x;
+    __shared__ double red[4];
+    __shared__ float turn[64][65];
+
+    double sum = 0.0;
+    for (unsigned i = tid; i < s.parts; i += 256) sum += b.partial[s.part + i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if ((tid & 63) == 0) red[tid >> 6] = sum;
+    __syncthreads();
+    const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
+    const double inv = (double)b.scale / (norm <= b.eps ? b.eps : norm);       // (a NaN norm stays)
+
+    const unsigned across = pad64(s.inner) / 64;
+    const int o0 = (int)(tile / across) * 64, i0 = (int)(tile % across) * 64;
+    const int m = s.inner_is_n ? s.outer : s.inner, n = s.inner_is_n ? s.inner : s.outer;
+    char* const base = b.ws + (size_t)s.base * 256;
+    char* const direct = base + buffer_offset(s.inner_is_n ? X : T0, m, n);
+    char* const turned = base + buffer_offset(s.inner_is_n ? T0 : X, m, n);
+    const unsigned lines_inner = pad64(s.inner) / 32, lines_outer = pad64(s.outer) / 32;
+    const float mu = MUON ? (hd ? hd->mom[s.group] : h.mom[s.group]) : 0.f;
+    const bool nest = MUON && b.nesterov;
+    const bool vec = s.dtype == 0 && s.si == 1 && (s.so & 3) == 0 && (s.inner & 3) == 0 && ((size_t)s.src & 15) == 0 && ((size_t)s.mom & 15) == 0;
+    const int c4 = (tid & 15) * 4;
+    for (int r = tid >> 4; r < 64; r += 16) {
+        const int o = o0 + r, i = i0 + c4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (o < s.outer) {
+            const long off = (long)o * s.so + (long)i * s.si;
+            if (vec) {
+                if (i < s.inner) {
+                    const float4 mv = MUON ? ld4(s.mom + off) : zero4();
+                    v[0] = mv.x; v[1] = mv.y; v[2] = mv.z; v[3] = mv.w;
+                    if (!MUON || nest) {
+                        const float4 gv = ld4(static_cast<const float*>(s.src) + off);
+                        v[0] = fmaf(mu, v[0], gv.x); v[1] = fmaf(mu, v[1], gv.y); v[2] = fmaf(mu, v[2], gv.z); v[3] = fmaf(mu, v[3], gv.w);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (i + x < s.inner) {
+                        const long at = off + x * s.si;
+                        if (MUON) {
+                            v[x] = s.mom[at];
+                            if (nest) v[x] = fmaf(mu, v[x], source_at(s, at));
+                        } else {
+                            v[x] = source_at(s, at);
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            v[x] = (float)((double)v[x] * inv);
+            turn[r][c4 + x] = v[x];
+        }
+        store4(direct, lines_inner, o, i, v);
+    }
+    __syncthreads();
+    for (int r = tid >> 4; r < 64; r += 16) {
+        float v[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = turn[c4 + x][r];
+        store4(turned, lines_outer, i0 + r, o0 + c4, v);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ products
+// One workgroup's BT x BT tile of L R^T over the lines q0 .. q1-1 of both operands: 4 waves in 2 x 2, two LDS stages of one line per
+// row.  LDS chunk c (16 B) of row r sits at c ^ ((r >> 1) & 7): 16 consecutive rows, which one ds_read_b128 phase reads, then
+// cover all 64 banks; the permutation is applied to the DMA's source address.
+template <int BT>
+struct Tile {
+    static constexpr int S = BT / 64;                    // 32 x 32 subtiles per wave and dimension
+    static constexpr unsigned STAGE = 2 * BT * LINE;
+    f32x16 acc[S][S];
+
+    __device__ __forceinline__ void run(char* smem, const char* L, unsigned rows_l, const char* R, unsigned rows_r, unsigned lines,
+                                        unsigned l0, unsigned r0, unsigned q0, unsigned q1) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int wr = wave >> 1, wc = wave & 1;
+        const unsigned pitch = lines * LINE;
+        const i32x4 rl = make_rsrc(L, rows_l * pitch), rr = make_rsrc(R, rows_r * pitch);
+        constexpr int PIECES = BT / 32;                  // 1 KiB pieces (8 rows) per wave and operand
+        unsigned off_l[PIECES], off_r[PIECES];
+        const unsigned lds = lds_addr(smem);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const unsigned row = (wave * PIECES + p) * 8 + (lane >> 3);
+            const unsigned chunk = (lane & 7) ^ ((row >> 1) & 7);
+            off_l[p] = (l0 + row) * pitch + chunk * 16;
+            off_r[p] = (r0 + row) * pitch + chunk * 16;
+        }
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.f;
+
+        auto issue = [&](unsigned q, unsigned stage) {
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) {
+                const unsigned at = lds + stage * STAGE + (wave * PIECES + p) * 1024;
+                dma16s(rl, off_l[p], q * LINE, at);
+                dma16s(rr, off_r[p], q * LINE, at + BT * LINE);
+            }
+        };
+        __syncthreads();                                 // the caller may have used this LDS
+        issue(q0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const int fr = lane & 31, fk = lane >> 5;
+        const int sw = (fr >> 1) & 7;                    // row bases are multiples of 32: the swizzle depends on the lane alone
+        for (unsigned q = q0; q < q1; ++q) {
+            const unsigned stage = (q - q0) & 1;
+            if (q + 1 < q1) issue(q + 1, stage ^ 1);
+            const char* const sl = smem + stage * STAGE + (wr * S * 32 + fr) * LINE;
+            const char* const sr = smem + stage * STAGE + BT * LINE + (wc * S * 32 + fr) * LINE;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const int hi = ((ks * 2 + fk) ^ sw) * 16, lo = ((ks * 2 + fk + 4) ^ sw) * 16;
+                f16x8 lh[S], ll[S], rh[S], rl8[S];
+#pragma unroll
+                for (int i = 0; i < S; ++i) {
+                    lh[i] = *reinterpret_cast<const f16x8*>(sl + i * 32 * LINE + hi);
+                    ll[i] = *reinterpret_cast<const f16x8*>(sl + i * 32 * LINE + lo);
+                    rh[i] = *reinterpret_cast<const f16x8*>(sr + i * 32 * LINE + hi);
+                    rl8[i] = *reinterpret_cast<const f16x8*>(sr + i * 32 * LINE + lo);
+                }
+#pragma unroll
+                for (int i = 0; i < S; ++i)
+#pragma unroll
+                    for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll[i], rh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < S; ++i)
+#pragma unroll
+                    for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[i], rl8[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < S; ++i)
+#pragma unroll
+                    for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[i], rh[j], acc[i][j], 0, 0, 0);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+    }
+
+    // f(i, j, g, row, col): values acc[i][j][4 g .. 4 g + 3] are rows row .. row+3 of column col (tile-relative)
+    template <typename F>
+    __device__ __forceinline__ void each4(F f) const {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int row = ((wave >> 1) * S + i) * 32 + 8 * g + 4 * (lane >> 5), col = ((wave & 1) * S + j) * 32 + (lane & 31);
+                    const float v[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                    f(row, col, v);
+                }
+    }
+};
+
+// t-th tile on or below the diagonal, row by row
+__device__ __forceinline__ void lower_tile(unsigned t, unsigned& i, unsigned& j) {
+    i = (unsigned)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while ((i + 1) * (i + 2) / 2 <= t) ++i;
+    while (i * (i + 1) / 2 > t) --i;
+    j = t - i * (i + 1) / 2;
+}
+
+// a symmetric result: rows r .. r+3 of column c, stored as values r .. r+3 of row c, and off the diagonal tiles also as themselves
+__device__ __forceinline__ void store_symmetric(char* out, unsigned lines, unsigned r, unsigned c, const float* v, bool mirror) {
+    store4(out, lines, c, r, v);
+    if (mirror) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) store1(out, lines, r + x, c, v[x]);
+    }
+}
+
+struct Product {
+    int l, r, out;
+    float scale;                     // fp32 sum -> stored result
+    float ident, lin;                // out = ident I + lin A + scale L R^T (POLY only; A in its stored scale)
+};
+struct ProductPair {
+    Product p[2];
+};
+
+// m x m products (all operands symmetric): A^2 with the polynomial's epilogue, Q A, W Q, P Q.  Two independent ones share a launch.
+template <int BT, bool POLY>
+__global__ __launch_bounds__(256, 2) void ns_square_product(Batch b, ProductPair pp) {
+    __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<BT>::STAGE];
+    const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
+    const Product pr = pp.p[blockIdx.y];
+    const Item s = b.item[find_item(b, wg)];
+    char* const base = b.ws + (size_t)s.base * 256;
+    const unsigned M = pad64(s.m), lines = M / 32;
+    unsigned ti, tj;
+    lower_tile(wg - s.first, ti, tj);
+    Tile<BT> t;
+    t.run(smem, base + buffer_offset(pr.l, s.m, s.n), M, base + buffer_offset(pr.r, s.m, s.n), M, lines, ti * BT, tj * BT, 0, lines);
+    char* const out = base + buffer_offset(pr.out, s.m, s.n);
+    const char* const a = base + buffer_offset(A, s.m, s.n);
+    t.each4([&](int row, int col, const float* acc) {
+        const unsigned r = ti * BT + row, c = tj * BT + col;
+        if (r >= M || c >= M) return;
+        float v[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = acc[x] * pr.scale;
+        if (POLY) {
+            float av[4];
+            load4(a, lines, c, r, av);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] += pr.lin * av[x] + (r + x == c && c < (unsigned)s.m ? pr.ident : 0.f);
+        }
+        store_symmetric(out, lines, r, c, v, ti != tj);
+    });
+}
+
+// Gram products A = X X^T: few tiles, long sums.  The sum is cut into `splits` runs of lines, each workgroup leaves its fp32 tile in
+// the workspace (as its registers lie, 16 B per lane), and ns_gram_reduce adds the runs in their order.
+struct GramItem {
+    unsigned first, part;            // workgroup of the launch; first tile slot in the partial region
+    int m, n;
+    unsigned base, tiles, splits, run;
+};
+struct GramBatch {
+    char* ws;
+    float* partial;
+    int count;
+    float scale;
+    GramItem item[BATCH];
+};
+
+template <int BT>
+__global__ __launch_bounds__(256, 2) void ns_gram(GramBatch b) {
+    __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<BT>::STAGE];
+    const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
+    const GramItem s = b.item[find_item(b, wg)];
+    const char* const x = b.ws + (size_t)s.base * 256;
+    const unsigned M = pad64(s.m), lines = pad64(s.n) / 32;
+    const unsigned u = wg - s.first, k = u / s.tiles, tile = u - k * s.tiles;      // the tiles of one run are neighbours: they share its lines
+    unsigned ti, tj;
+    lower_tile(tile, ti, tj);
+    Tile<BT> t;
+    const unsigned q0 = k * s.run, q1 = q0 + s.run < lines ? q0 + s.run : lines;
+    t.run(smem, x, M, x, M, lines, ti * BT, tj * BT, q0, q1);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    constexpr int S = Tile<BT>::S;
+    float* const out = b.partial + ((size_t)s.part + (size_t)tile * s.splits + k) * (BT * BT);
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int sub = ((wave >> 1) * S + i) * (BT / 32) + (wave & 1) * S + j;
+                st4(out + (((size_t)sub * 4 + g) * 64 + lane) * 4,
+                    make_float4(t.acc[i][j][4 * g], t.acc[i][j][4 * g + 1], t.acc[i][j][4 * g + 2], t.acc[i][j][4 * g + 3]));
+            }
+}
+
+// one workgroup per 32 x 32 subtile; wave w adds the runs w, w + 4, ... and the four sums are joined in order
+template <int BT>
+__global__ __launch_bounds__(256) void ns_gram_reduce(GramBatch b) {
+    constexpr unsigned SUBS = (BT / 32) * (BT / 32);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    // `first` counts the product's workgroups (tiles * splits): this launch has tiles * SUBS per item, so the item is found by walking
+    unsigned wg = blockIdx.x;
+    int it = 0;
+    while (wg >= b.item[it].tiles * SUBS) wg -= b.item[it++].tiles * SUBS;
+    const GramItem s = b.item[it];
+    const unsigned tile = wg / SUBS, sub = wg - tile * SUBS;
+    const float* const in = b.partial + ((size_t)s.part + (size_t)tile * s.splits) * (BT * BT) + (size_t)sub * 1024 + lane * 4;
+    float4 v[4] = {zero4(), zero4(), zero4(), zero4()};
+    for (unsigned k = wave; k < s.splits; k += 4)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 p = ld4(in + (size_t)k * (BT * BT) + g * 256);
+            v[g].x += p.x; v[g].y += p.y; v[g].z += p.z; v[g].w += p.w;
+        }
+    __shared__ float4 red[4][4][64];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) red[wave][g][lane] = v[g];
+    __syncthreads();
+    const int g = wave;                                  // wave g joins and stores register group g
+    const float4 a = red[0][g][lane], c = red[1][g][lane], d = red[2][g][lane], e = red[3][g][lane];
+    const float r4[4] = {((a.x + c.x) + (d.x + e.x)) * b.scale, ((a.y + c.y) + (d.y + e.y)) * b.scale,
+                         ((a.z + c.z) + (d.z + e.z)) * b.scale, ((a.w + c.w) + (d.w + e.w)) * b.scale};
+    unsigned ti, tj;
+    lower_tile(tile, ti, tj);
+    const unsigned M = pad64(s.m);
+    const unsigned row = ti * BT + (sub / (BT / 32)) * 32 + 8 * g + 4 * (lane >> 5), col = tj * BT + (sub % (BT / 32)) * 32 + (lane & 31);
+    if (row >= M || col >= M) return;
+    store_symmetric(b.ws + (size_t)s.base * 256 + buffer_offset(A, s.m, s.n), M / 32, row, col, r4, ti != tj);
+}
+
+// X <- P X between segments: both orders again (T1 from T0, X in place: no workgroup reads X)
+template <int BT>
+__global__ __launch_bounds__(256, 2) void ns_apply(Batch b, int p, int tin, int tout, float scale) {
+    __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<BT>::STAGE];
+    const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
+    const Item s = b.item[find_item(b, wg)];
+    char* const base = b.ws + (size_t)s.base * 256;
+    const unsigned M = pad64(s.m), N = pad64(s.n);
+    const unsigned down = (M + BT - 1) / BT, u = wg - s.first, tj = u / down, ti = u - tj * down;
+    Tile<BT> t;
+    t.run(smem, base + buffer_offset(p, s.m, s.n), M, base + buffer_offset(tin, s.m, s.n), N, M / 32, ti * BT, tj * BT, 0, M / 32);
+    char* const xo = base;
+    char* const to = base + buffer_offset(tout, s.m, s.n);
+    t.each4([&](int row, int col, const float* acc) {
+        const unsigned r = ti * BT + row, c = tj * BT + col;
+        if (r >= M || c >= N) return;
+        float v[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = acc[x] * scale;
+        store4(to, M / 32, c, r, v);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) store1(xo, N / 32, r + x, c, v[x]);
+    });
+}
+
+// the last product goes straight to where the caller wants it
+struct Target {
+    unsigned first, base;
+    void* dst;
+    long si, sj;                     // strides of X's rows (m) and columns (n) in the destination
+    int m, n;
+    float factor;                    // MUON: the shape's factor on lr
+    int dtype, group;
+    int turned;                      // 1: the lanes of a wave run along m (si == 1)
+};
+struct TargetBatch {
+    char* ws;
+    int count;
+    int p, tin;
+    float scale;
+    Target item[BATCH];
+};
+
+// MUON: param = param (1 - lr wd) - lr factor O, else dst = O
+template <int BT, bool MUON>
+__global__ __launch_bounds__(256, 2) void ns_finish(TargetBatch b, Hyper h, const Hyper* __restrict__ hd) {
+    __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<BT>::STAGE];
+    const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
+    const Target s = b.item[find_item(b, wg)];
+    const char* const base = b.ws + (size_t)s.base * 256;
+    const unsigned M = pad64(s.m), N = pad64(s.n);
+    const unsigned down = (M + BT - 1) / BT, u = wg - s.first, tj = u / down, ti = u - tj * down;
+    const char* const P = base + buffer_offset(b.p, s.m, s.n);
+    const char* const T = base + buffer_offset(b.tin, s.m, s.n);
+    Tile<BT> t;
+    if (s.turned) t.run(smem, T, N, P, M, M / 32, tj * BT, ti * BT, 0, M / 32);
+    else t.run(smem, P, M, T, N, M / 32, ti * BT, tj * BT, 0, M / 32);
+    const unsigned r0 = (s.turned ? tj : ti) * BT, c0 = (s.turned ? ti : tj) * BT;
+    const unsigned rows = s.turned ? s.n : s.m, cols = s.turned ? s.m : s.n;
+    const long sr = s.turned ? s.sj : s.si, sc = s.turned ? s.si : s.sj;
+    float keep = 1.f, step = 0.f;
+    if (MUON) {
+        const float lr = hd ? hd->lr[s.group] : h.lr[s.group], wd = hd ? hd->wd[s.group] : h.wd[s.group];
+        keep = 1.f - lr * wd;
+        step = lr * s.factor * b.scale;
+    }
+    t.each4([&](int row, int col, const float* acc) {
+        const unsigned c = c0 + col;
+        if (c >= cols) return;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const unsigned r = r0 + row + x;
+            if (r >= rows) break;
+            const long at = (long)r * sr + (long)c * sc;
+            if (MUON) {
+                float* const p = static_cast<float*>(s.dst) + at;
+                *p = fmaf(-step, acc[x], *p * keep);
+            } else if (s.dtype) {
+                static_cast<unsigned short*>(s.dst)[at] = f32_to_bf16(acc[x] * b.scale);
+            } else {
+                static_cast<float*>(s.dst)[at] = acc[x] * b.scale;
+            }
+        }
+    });
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+// Largest value of |f| on [0, s] for the polynomials of the iteration, and the power-of-two scale that keeps such entries below 2^15
+// (fp16 ends at 65504; a matrix's entries are bounded by its spectral norm).
+struct Bounds {
+    double a, b, c;
+    static float scale_for(double bound) {
+        int e;
+        std::frexp(32768.0 / bound, &e);                 // 32768 / bound in [2^(e-1), 2^e)
+        return (float)std::ldexp(1.0, e - 1);
+    }
+    double p(double s) const { return std::fabs(s * (a + s * s * (b + s * s * c))); }
+    double q(double s) const { return std::fabs(a + s * s * (b + s * s * c)); }
+    double max_p(double s) const {
+        double v = p(s);
+        // p' = a + 3 b y + 5 c y^2, y = s^2
+        double y[2];
+        int k = 0;
+        if (c != 0.0) {
+            const double d = 9.0 * b * b - 20.0 * a * c;
+            if (d >= 0.0) {
+                y[k++] = (-3.0 * b + std::sqrt(d)) / (10.0 * c);
+                y[k++] = (-3.0 * b - std::sqrt(d)) / (10.0 * c);
+            }
+        } else if (b != 0.0) {
+            y[k++] = -a / (3.0 * b);
+        }
+        while (k-- > 0)
+            if (y[k] > 0.0 && y[k] < s * s) v = std::fmax(v, p(std::sqrt(y[k])));
+        return v;
+    }
+    double max_q(double s) const {
+        double v = std::fmax(q(0.0), q(s));
+        if (c != 0.0) {
+            const double y = -b / (2.0 * c);
+            if (y > 0.0 && y < s * s) v = std::fmax(v, q(std::sqrt(y)));
+        }
+        return v;
+    }
+};
+constexpr double SLACK = 1.0 + 1e-5;                     // what rounding may add to a bound
+constexpr double MAX_BOUND = 4096.0;                     // coefficients whose iterates grow beyond this are refused
+
+// 2, 1, 2, 1, ... steps between Gram products, see the head of this file
+int segment_length(int index, int left) { return (index & 1) == 0 && left >= 2 ? 2 : 1; }
+
+bool iteration_ok(const Bounds& f, int steps) {
+    double s = SLACK;
+    for (int left = steps, seg = 0; left > 0; ++seg) {
+        double P = 1.0;
+        for (int i = segment_length(seg, left); i > 0; --i, --left) {
+            P *= f.max_q(s) * SLACK;
+            s = f.max_p(s) * SLACK;
+            if (!(P > 1e-6 && P < MAX_BOUND && s > 1e-6 && s < MAX_BOUND)) return false;
+        }
+    }
+    return true;
+}
+
+struct Shape {
+    int m, n;                        // m <= n
+    int outer, inner;                // as the source lies
+};
+
+struct Plan {
+    size_t partial_at, gram_at, mats_at, bytes;
+};
+
+constexpr int BT = 64;
+
+unsigned tiles_of(int m) { return pad64(m) / BT; }
+
+// runs of a Gram product: enough workgroups to fill the chip, no run shorter than 8 lines
+unsigned gram_run(const Shape* s, int count) {
+    double work = 0.0;
+    for (int i = 0; i < count; ++i) {
+        const unsigned t = tiles_of(s[i].m);
+        work += (double)(t * (t + 1) / 2) * (pad64(s[i].n) / 32);
+    }
+    const double run = std::ceil(work / 2048.0);
+    return run < 8.0 ? 8u : (unsigned)run;
+}
+
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+Plan plan_batch(const Shape* s, int count) {
+    Plan p;
+    size_t parts = 0, slots = 0, mats = 0;
+    const unsigned run = gram_run(s, count);
+    for (int i = 0; i < count; ++i) {
+        const unsigned t = tiles_of(s[i].m), lines = pad64(s[i].n) / 32;
+        parts += (size_t)segmi_cdiv(s[i].outer, 64) * segmi_cdiv(s[i].inner, 256);
+        slots += (size_t)(t * (t + 1) / 2) * segmi_cdiv(lines, run);
+        mats += 3 * big_bytes(s[i].m, s[i].n) + 5 * square_bytes(s[i].m);
+    }
+    p.partial_at = 0;
+    p.gram_at = align256(parts * sizeof(double));
+    p.mats_at = p.gram_at + align256(slots * BT * BT * sizeof(float));
+    p.bytes = p.mats_at + mats;
+    return p;
+}
+
+// runs the whole iteration of up to BATCH matrices; `src` and `dst` carry the callers' pointers, the rest is filled in here
+template <bool MUON>
+int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count, const Bounds& f, int steps, char* ws,
+              const Hyper& h, const Hyper* hd, hipStream_t st) {
+    const Plan plan = plan_batch(shapes, count);
+    const unsigned run = gram_run(shapes, count);
+    Batch sq, big;
+    GramBatch gram;
+    src.ws = dst.ws = sq.ws = big.ws = gram.ws = ws + plan.mats_at;
+    src.partial = reinterpret_cast<double*>(ws + plan.partial_at);
+    gram.partial = reinterpret_cast<float*>(ws + plan.gram_at);
+    src.count = dst.count = sq.count = big.count = gram.count = count;
+
+    unsigned g_sum = 0, g_norm = 0, g_sq = 0, g_gram = 0, g_red = 0, g_big = 0, parts = 0, slots = 0;
+    size_t base = 0;
+    for (int i = 0; i < count; ++i) {
+        const Shape& s = shapes[i];
+        const unsigned t = tiles_of(s.m), lines = pad64(s.n) / 32, low = t * (t + 1) / 2, splits = segmi_cdiv(lines, run);
+        const unsigned b256 = (unsigned)(base / 256);
+        const unsigned units = segmi_cdiv(s.outer, 64) * segmi_cdiv(s.inner, 256);
+        src.item[i].base = dst.item[i].base = b256;
+        src.item[i].first = g_sum;
+        src.item[i].part = parts;
+        src.item[i].parts = units;
+        sq.item[i] = Item{g_sq, s.m, s.n, b256};
+        gram.item[i] = GramItem{g_gram, slots, s.m, s.n, b256, low, splits, run};
+        big.item[i] = Item{g_big, s.m, s.n, b256};
+        dst.item[i].first = g_big;
+        g_sum += units;
+        parts += units;
+        g_norm += (pad64(s.outer) / 64) * (pad64(s.inner) / 64);
+        g_sq += low;
+        g_gram += low * splits;
+        g_red += low * (BT / 32) * (BT / 32);
+        slots += low * splits;
+        g_big += t * (pad64(s.n) / BT);
+        base += 3 * big_bytes(s.m, s.n) + 5 * square_bytes(s.m);
+    }
+    hipLaunchKernelGGL((ns_sum_squares<MUON>), dim3(g_sum), dim3(256), 0, st, src, h, hd);
+    unsigned at = 0;
+    for (int i = 0; i < count; ++i) {
+        src.item[i].first = at;
+        at += (pad64(shapes[i].outer) / 64) * (pad64(shapes[i].inner) / 64);
+    }
+    double s = SLACK;                                    // bound of X's singular values
+    double sx = Bounds::scale_for(s);
+    src.scale = (float)sx;
+    hipLaunchKernelGGL((ns_normalise<MUON>), dim3(g_norm), dim3(256), 0, st, src, h, hd);
+
+    int tin = T0;
+    for (int left = steps, seg = 0; left > 0; ++seg) {
+        const int len = segment_length(seg, left);
+        double sa = Bounds::scale_for(s * s);
+        gram.scale = (float)(sa / (sx * sx));
+        hipLaunchKernelGGL((ns_gram<BT>), dim3(g_gram), dim3(256), 0, st, gram);
+        hipLaunchKernelGGL((ns_gram_reduce<BT>), dim3(g_red), dim3(256), 0, st, gram);
+        int p = P0;
+        double bp = 1.0, sp = 1.0;
+        for (int i = 0; i < len; ++i) {
+            const double bq = f.max_q(s) * SLACK, bnext = f.max_p(s) * SLACK, bw = s * bnext;
+            const double sqs = Bounds::scale_for(bq);
+            const int qbuf = i == 0 ? P0 : Q;            // the first Q of a segment is its P
+            ProductPair pp;
+            pp.p[0] = Product{A, A, qbuf, (float)(f.c * sqs / (sa * sa)), (float)(f.a * sqs), (float)(f.b * sqs / sa)};
+            pp.p[1] = pp.p[0];
+            hipLaunchKernelGGL((ns_square_product<BT, true>), dim3(g_sq), dim3(256), 0, st, sq, pp);
+            int two = 0;
+            if (i == 0) {
+                bp = bq;
+                sp = sqs;
+            } else {
+                const double nsp = Bounds::scale_for(bp * bq);
+                const int np = p == P0 ? P1 : P0;
+                pp.p[two++] = Product{p, Q, np, (float)(nsp / (sp * sqs)), 0.f, 0.f};
+                bp *= bq;
+                sp = nsp;
+                p = np;
+            }
+            const double sw = Bounds::scale_for(bw), san = Bounds::scale_for(bnext * bnext);
+            if (i + 1 < len) pp.p[two++] = Product{qbuf, A, W, (float)(sw / (sqs * sa)), 0.f, 0.f};
+            if (two) hipLaunchKernelGGL((ns_square_product<BT, false>), dim3(g_sq, two), dim3(256), 0, st, sq, pp);
+            if (i + 1 < len) {
+                pp.p[0] = Product{W, qbuf, A, (float)(san / (sw * sqs)), 0.f, 0.f};
+                hipLaunchKernelGGL((ns_square_product<BT, false>), dim3(g_sq), dim3(256), 0, st, sq, pp);
+                sa = san;
+            }
+            s = bnext;
+        }
+        left -= len;
+        if (left > 0) {
+            const double nsx = Bounds::scale_for(s);
+            const int tout = tin == T0 ? T1 : T0;
+            hipLaunchKernelGGL((ns_apply<BT>), dim3(g_big), dim3(256), 0, st, big, p, tin, tout, (float)(nsx / (sp * sx)));
+            tin = tout;
+            sx = nsx;
+        } else {
+            dst.p = p;
+            dst.tin = tin;
+            dst.scale = (float)(1.0 / (sp * sx));
+            hipLaunchKernelGGL((ns_finish<BT, MUON>), dim3(g_big), dim3(256), 0, st, dst, h, hd);
+        }
+    }
+    return segmi_launch_status();
+}
+
+bool shape_ok(int rows, int cols) {
+    return rows > 0 && cols > 0 && big_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows) < ((size_t)1 << 32);
+}
+
+// `inner` = the contiguous dimension
+Shape shape_of(int rows, int cols, bool cols_inner) {
+    return Shape{rows <= cols ? rows : cols, rows <= cols ? cols : rows, cols_inner ? rows : cols, cols_inner ? cols : rows};
+}
+
+Shape shape_of(const segmi_ns_matrix& a) { return shape_of(a.rows, a.cols, a.src_cs == 1 || a.src_rs != 1); }
+
+// workspace of a call: its batches run one after the other and share it
+template <typename M, typename F>
+size_t workspace_of(const M* mats, int count, F shape) {
+    size_t most = 0;
+    Shape s[BATCH];
+    for (int at = 0; at < count; at += BATCH) {
+        const int k = count - at < BATCH ? count - at : BATCH;
+        for (int i = 0; i < k; ++i) s[i] = shape(mats[at + i]);
+        const Plan p = plan_batch(s, k);
+        if (p.bytes > most) most = p.bytes;
+    }
+    return most;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t segmi_ns_workspace(const segmi_ns_matrix* mats_host, int count) {
+    if (!mats_host || count <= 0) return 0;
+    for (int i = 0; i < count; ++i)
+        if (!shape_ok(mats_host[i].rows, mats_host[i].cols)) return 0;
+    return workspace_of(mats_host, count, [](const segmi_ns_matrix& a) { return shape_of(a); });
+}
+
+int segmi_ns_coefficients_ok(const double* coefficients_host, int steps) {
+    if (!coefficients_host || steps < 1 || steps > SEGMI_NS_MAX_STEPS) return 0;
+    return iteration_ok(Bounds{coefficients_host[0], coefficients_host[1], coefficients_host[2]}, steps) ? 1 : 0;
+}
+
+int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const double* coefficients_host, int steps, double eps,
+                           void* workspace, size_t workspace_bytes, segmi_stream_t stream) {
+    if (!mats_host || count <= 0 || !(eps > 0.0) || !workspace || !segmi_ns_coefficients_ok(coefficients_host, steps)) return SEGMI_ERR_BADARG;
+    for (int i = 0; i < count; ++i) {
+        const segmi_ns_matrix& a = mats_host[i];
+        if (!a.src || !a.dst || !shape_ok(a.rows, a.cols) || a.dtype < 0 || a.dtype > 1) return SEGMI_ERR_BADARG;
+    }
+    if ((size_t)workspace & 255) return SEGMI_ERR_ALIGN;
+    if (workspace_bytes < segmi_ns_workspace(mats_host, count)) return SEGMI_ERR_WORKSPACE;
+    const Bounds f{coefficients_host[0], coefficients_host[1], coefficients_host[2]};
+    for (int at = 0; at < count; at += BATCH) {
+        const int k = count - at < BATCH ? count - at : BATCH;
+        Shape shapes[BATCH];
+        SourceBatch src{};
+        TargetBatch dst{};
+        src.eps = eps;
+        for (int i = 0; i < k; ++i) {
+            const segmi_ns_matrix& a = mats_host[at + i];
+            const Shape s = shapes[i] = shape_of(a);
+            const bool cols_inner = a.src_cs == 1 || a.src_rs != 1, wide = a.rows <= a.cols;
+            Source& o = src.item[i];
+            o.src = a.src;
+            o.so = cols_inner ? a.src_rs : a.src_cs;
+            o.si = cols_inner ? a.src_cs : a.src_rs;
+            o.outer = s.outer;
+            o.inner = s.inner;
+            o.dtype = a.dtype;
+            o.inner_is_n = cols_inner == wide;
+            Target& t = dst.item[i];
+            t.dst = a.dst;
+            t.si = wide ? a.dst_rs : a.dst_cs;
+            t.sj = wide ? a.dst_cs : a.dst_rs;
+            t.m = s.m;
+            t.n = s.n;
+            t.dtype = a.dtype;
+            t.turned = t.si == 1 && t.sj != 1;
+        }
+        const int rc = run_batch<false>(shapes, src, dst, k, f, steps, static_cast<char*>(workspace), Hyper{}, nullptr, (hipStream_t)stream);
+        if (rc != SEGMI_OK) return rc;
+    }
+    return SEGMI_OK;
+}
+
+size_t segmi_muon_workspace(const segmi_muon_matrix* mats_host, int count) {
+    if (!mats_host || count <= 0) return 0;
+    for (int i = 0; i < count; ++i)
+        if (!shape_ok(mats_host[i].rows, mats_host[i].cols)) return 0;
+    return workspace_of(mats_host, count, [](const segmi_muon_matrix& a) { return shape_of(a.rows, a.cols, true); });
+}
+
+int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* lr_host, const float* weight_decay_host,
+                    const float* momentum_host, int ngroups, const float* hyper_dev, int nesterov, const double* coefficients_host, int steps,
+                    double eps, void* workspace, size_t workspace_bytes, segmi_stream_t stream) {
+    if (!mats_host || count <= 0 || !(eps > 0.0) || !workspace || !segmi_ns_coefficients_ok(coefficients_host, steps)) return SEGMI_ERR_BADARG;
+    if (!hyper_dev && (!lr_host || !weight_decay_host || !momentum_host)) return SEGMI_ERR_BADARG;
+    if (ngroups <= 0 || ngroups > MAX_GROUPS) return SEGMI_ERR_BADARG;
+    for (int i = 0; i < count; ++i) {
+        const segmi_muon_matrix& a = mats_host[i];
+        if (!a.param || !a.grad || !a.momentum || !shape_ok(a.rows, a.cols) || a.group < 0 || a.group >= ngroups) return SEGMI_ERR_BADARG;
+    }
+    if ((size_t)workspace & 255) return SEGMI_ERR_ALIGN;
+    if (workspace_bytes < segmi_muon_workspace(mats_host, count)) return SEGMI_ERR_WORKSPACE;
+    const Bounds f{coefficients_host[0], coefficients_host[1], coefficients_host[2]};
+    Hyper h{};
+    if (!hyper_dev)
+        for (int i = 0; i < ngroups; ++i) {
+            h.lr[i] = lr_host[i];
+            h.wd[i] = weight_decay_host[i];
+            h.mom[i] = momentum_host[i];
+        }
+    for (int at = 0; at < count; at += BATCH) {
+        const int k = count - at < BATCH ? count - at : BATCH;
+        Shape shapes[BATCH];
+        SourceBatch src{};
+        TargetBatch dst{};
+        src.eps = eps;
+        src.nesterov = nesterov;
+        for (int i = 0; i < k; ++i) {
+            const segmi_muon_matrix& a = mats_host[at + i];
+            const Shape s = shapes[i] = shape_of(a.rows, a.cols, true);
+            const bool wide = a.rows <= a.cols;
+            Source& o = src.item[i];
+            o.src = a.grad;
+            o.mom = a.momentum;
+            o.so = a.cols;
+            o.si = 1;
+            o.outer = s.outer;
+            o.inner = s.inner;
+            o.inner_is_n = wide;
+            o.group = a.group;
+            Target& t = dst.item[i];
+            t.dst = a.param;
+            t.si = wide ? a.cols : 1;
+            t.sj = wide ? 1 : a.cols;
+            t.m = s.m;
+            t.n = s.n;
+            t.factor = a.factor;
+            t.group = a.group;
+            t.turned = !wide;
+        }
+        const int rc = run_batch<true>(shapes, src, dst, k, f, steps, static_cast<char*>(workspace), h,
+                                       reinterpret_cast<const Hyper*>(hyper_dev), (hipStream_t)stream);
+        if (rc != SEGMI_OK) return rc;
+    }
+    return SEGMI_OK;
+}
+
+}  // extern "C"

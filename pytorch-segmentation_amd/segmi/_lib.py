@@ -141,6 +141,12 @@ SIGNATURES = {
     "segmi_sgd_step": (i32, [vp, i32, vp, vp, vp, i32, vp]),
     "segmi_sgd_hyper_floats": (i32, []),
     "segmi_sgd_step_dev": (i32, [vp, i32, vp, vp]),
+    "segmi_ns_workspace": (sz, [vp, i32]),
+    "segmi_ns_coefficients_ok": (i32, [vp, i32]),
+    "segmi_ns_orthogonalize": (i32, [vp, i32, vp, i32, C.c_double, vp, sz, vp]),
+    "segmi_muon_workspace": (sz, [vp, i32]),
+    "segmi_muon_step": (i32, [vp, i32, vp, vp, vp, i32, vp, i32, vp, i32, C.c_double, vp, sz, vp]),
+    "segmi_adamw_step": (i32, [vp, i32, vp, i32, vp, vp, sz, vp]),
     "segmi_pyramid_pool_workspace": (sz, [i32, i32, i32, i32, i32, vp]),
     "segmi_pyramid_pool_fwd": (i32, [vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, sz, vp]),
     "segmi_pyramid_pool_bwd": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, sz, vp]),

@@ -1,0 +1,446 @@
+"""The optimizer of large language models on libsegmi: orthogonalised updates for matrices, AdamW for everything else.
+
+`orthogonalize`  replaces matrices by their nearest (semi-)orthogonal ones, by Newton-Schulz products.
+`Muon`           momentum -> orthogonalize -> update for every parameter that is a matrix (convolution filters [K, C, R, S] are
+                 K x C*R*S), AdamW for the rest (norms, biases, depthwise filters).  One optimizer for a whole network.
+`FusedAdamW`     AdamW alone.
+
+All three are reached through `segmi.optim`, and the two optimizers by name from config.json (`"optimizer": {"type": "Muon", ...}`), the
+way the reference resolves its optimizers (`base/base_trainer.py:57`).  `AdamW` in a config stays torch.optim.AdamW.
+Pointers travel as kernel arguments: no table is uploaded, gradients may move between steps, nothing waits for the GPU.
+"""
+import ctypes as C
+import math
+
+import numpy as np
+import torch
+
+from ._lib import SegmiError, check, lib
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+_NS_DTYPE = np.dtype([("src", "<u8"), ("dst", "<u8"), ("src_rs", "<i8"), ("src_cs", "<i8"), ("dst_rs", "<i8"), ("dst_cs", "<i8"),
+                      ("rows", "<i4"), ("cols", "<i4"), ("dtype", "<i4"), ("reserved", "<i4")])
+_MUON_DTYPE = np.dtype([("param", "<u8"), ("grad", "<u8"), ("momentum", "<u8"), ("rows", "<i4"), ("cols", "<i4"), ("factor", "<f4"), ("group", "<i4")])
+_ADAMW_DTYPE = np.dtype([("param", "<u8"), ("grad", "<u8"), ("exp_avg", "<u8"), ("exp_avg_sq", "<u8"), ("step_dev", "<u8"), ("step", "<f8"),
+                         ("count", "<i8"), ("group", "<i4"), ("reserved", "<i4")])
+_MAX_GROUPS = 8
+_ADAMW_HYPER = 5                              # lr, weight decay, beta 1, beta 2, eps
+
+
+def _check_iteration(steps, coefficients, eps, what):
+    if isinstance(steps, bool) or int(steps) != steps or not 1 <= steps <= 32:
+        raise ValueError("%s: the number of Newton-Schulz steps must be an integer in 1..32, got %r" % (what, steps))
+    coefficients = tuple(float(c) for c in coefficients)
+    if len(coefficients) != 3:
+        raise ValueError("%s: three Newton-Schulz coefficients (a, b, c) are needed, got %d" % (what, len(coefficients)))
+    if not (float(eps) > 0.0 and math.isfinite(eps)):
+        raise ValueError("%s: eps must be positive and finite, got %r" % (what, eps))
+    arr = (C.c_double * 3)(*coefficients)
+    if not all(math.isfinite(c) for c in coefficients) or not lib.segmi_ns_coefficients_ok(arr, int(steps)):
+        raise ValueError("%s: with coefficients %r the singular values do not stay bounded over %d steps" % (what, coefficients, steps))
+    return arr
+
+
+def _unit_of(sizes, strides):
+    """The stride u of the densely packed run these dimensions form (in any order), or None."""
+    dims = sorted((st, n) for n, st in zip(sizes, strides) if n > 1)
+    if not dims:
+        return 1
+    unit = expect = dims[0][0]
+    for st, n in dims:
+        if st != expect:
+            return None
+        expect = st * n
+    return unit if unit > 0 else None
+
+
+def _matrix_strides(t):
+    """(row stride, column stride) of t seen as shape[0] x rest, columns in the order of memory; None if it has none."""
+    cs = t.stride(1) if t.dim() == 2 else _unit_of(t.shape[1:], t.stride()[1:])
+    return None if cs is None else (t.stride(0), cs)
+
+
+@torch.no_grad()
+def orthogonalize(matrices, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
+    """X = M / max(|M|_F, eps), then `steps` times X <- (a I + b X X^T + c (X X^T)^2) X on the shorter side: all singular values
+    of M go to about 1.
+
+    `matrices`: a float32 or bfloat16 CUDA tensor of two or more dimensions (seen as shape[0] x the rest), or a list of them, any sizes
+    and strides; all of them share the launches.  Returns new tensors of the same shapes, types and (where dense) strides.  Computed
+    to fp32 accuracy in both types.  No gradient is recorded.  A matrix that holds NaN or infinity comes back as NaN, a zero one as zero.
+    Runs on the current stream of the tensors' device; may be captured into a hipGraph."""
+    single = isinstance(matrices, torch.Tensor)
+    mats = [matrices] if single else list(matrices)
+    coef = _check_iteration(steps, coefficients, eps, "segmi.optim.orthogonalize")
+    outs, rows = [], []
+    keep = []                                     # copies of inputs without a matrix order live until the launches are queued
+    device = None
+    for t in mats:
+        if not isinstance(t, torch.Tensor) or t.dim() < 2:
+            raise ValueError("segmi.optim.orthogonalize: a tensor of two or more dimensions is needed, got %s" %
+                             (tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__,))
+        if not t.is_cuda:
+            raise SegmiError("segmi.optim.orthogonalize: tensor is on %s — the kernels only run on the MI355X (there is deliberately no "
+                             "CPU / eager fallback)" % t.device)
+        if t.dtype not in (torch.float32, torch.bfloat16):
+            raise SegmiError("segmi.optim.orthogonalize: expected float32 or bfloat16, got %s" % t.dtype)
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise SegmiError("segmi.optim.orthogonalize: all matrices must be on one device, got %s and %s" % (device, t.device))
+        out = torch.empty_like(t)
+        outs.append(out)
+        if t.numel() == 0:
+            continue
+        st = _matrix_strides(t)
+        if st is None or (t.dim() > 2 and out.stride() != t.stride()):
+            t = t.contiguous()
+            keep.append(t)
+            out = outs[-1] = torch.empty_like(t)
+            st = _matrix_strides(t)
+        so = _matrix_strides(out)
+        r = t.shape[0]
+        rows.append((t.data_ptr(), out.data_ptr(), st[0], st[1], so[0], so[1], r, t.numel() // r, 0 if t.dtype == torch.float32 else 1, 0))
+    if rows:
+        desc = np.array(rows, dtype=_NS_DTYPE)
+        with torch.cuda.device(device):
+            nbytes = lib.segmi_ns_workspace(desc.ctypes.data, len(rows))
+            if not nbytes:
+                raise SegmiError("segmi.optim.orthogonalize: a matrix is too large (4 GiB of float32 after padding its sides to 64)")
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            check(lib.segmi_ns_orthogonalize(desc.ctypes.data, len(rows), coef, int(steps), float(eps), ws.data_ptr(), nbytes,
+                                             torch.cuda.current_stream().cuda_stream), "ns_orthogonalize")
+    return outs[0] if single else outs
+
+
+def _same_layout(a, b):
+    return a.shape == b.shape and all(sa == sb or n == 1 for sa, sb, n in zip(a.stride(), b.stride(), a.shape))
+
+
+class _Hyper:
+    """Per-group numbers in device memory (graphs): a ring of pinned slots and stream-ordered copies, as segmi.optim.SGD's."""
+    RING = 8
+
+    def __init__(self, nbytes, device):
+        self.slots = torch.zeros(self.RING, nbytes, dtype=torch.uint8).pin_memory()
+        self.events = [None] * self.RING
+        self.dev = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        self.at = 0
+
+    def push(self, values):
+        i, self.at = self.at, (self.at + 1) % self.RING
+        if self.events[i] is not None:
+            self.events[i].synchronize()             # the copy that last read this slot has executed
+        self.slots[i].copy_(torch.from_numpy(values))
+        self.dev.copy_(self.slots[i], non_blocking=True)
+        self.events[i] = torch.cuda.Event()
+        self.events[i].record()
+
+
+class _FusedOptimizer(torch.optim.Optimizer):
+    """What both optimizers share: state buffers in the parameters' memory order, descriptors that are rebuilt only when a pointer
+    moved, step numbers, capture."""
+
+    def __init__(self, params, defaults, capturable):
+        super().__init__(params, defaults)
+        self.capturable = bool(capturable)
+        self._hyper = None
+        self._sig = {}
+        self._desc = {}
+        self._steps = self._step_of = None           # one flat tensor of step numbers; state[p]["step"] are views of it
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        if len(self.param_groups) > _MAX_GROUPS:
+            self.param_groups.pop()
+            raise ValueError("%s supports up to %d parameter groups" % (self._name(), _MAX_GROUPS))
+
+    def _name(self):
+        return "segmi.optim." + type(self).__name__
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but the buffers become this optimizer's own: torch keeps the tensors of the dictionary where type and device fit,
+        and the kernels here would advance those of the optimizer it came from as well."""
+        super().load_state_dict(state_dict)
+        for st in self.state.values():
+            for key, v in st.items():
+                if isinstance(v, torch.Tensor):
+                    st[key] = v.clone()
+        self._sig.clear()
+
+    def _buffer(self, p, key):
+        """state[p][key] in p's own memory order; created, or re-laid once if it arrived in another (a loaded state_dict)."""
+        st = self.state[p]
+        buf = st.get(key)
+        if buf is None:
+            buf = st[key] = torch.zeros_like(p, memory_format=torch.preserve_format)
+        elif not (buf.shape == p.shape and _same_layout(buf, p) and buf.device == p.device and buf.dtype == p.dtype):
+            if buf.shape != p.shape:
+                raise RuntimeError("%s: %s has shape %s for a parameter of shape %s" % (self._name(), key, tuple(buf.shape), tuple(p.shape)))
+            fixed = torch.empty_like(p, memory_format=torch.preserve_format)
+            fixed.copy_(buf)
+            buf = st[key] = fixed
+        return buf
+
+    def _checked(self, p):
+        g = p.grad
+        if not (p.is_cuda and p.dtype == torch.float32 and not g.is_sparse and g.dtype == torch.float32 and g.device == p.device and
+                _same_layout(g, p) and _unit_of(p.shape, p.stride()) == 1):
+            raise RuntimeError("%s: parameters and gradients must be float32 CUDA tensors on one device with identical (dense) strides" % self._name())
+        if p.device != self._device():
+            raise RuntimeError("%s: all parameters must be on one device, got %s and %s" % (self._name(), self._device(), p.device))
+        return g
+
+    def _device(self):
+        return self.param_groups[0]["params"][0].device
+
+    def _adamw_descriptors(self, members):
+        """members: [(group index, parameter)] with gradients.  Descriptor array of segmi_adamw_step with this step's numbers."""
+        state = self.state
+        sig = []
+        for gi, p in members:
+            st = state[p]
+            if "exp_avg" in st and "exp_avg_sq" in st:
+                sig.append((p.data_ptr(), p.grad.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), id(st.get("step")), gi))
+            else:
+                sig.append(None)
+        if sig != self._sig.get("adamw"):
+            self._refuse_rebuild_in_capture()
+            rows = []
+            for gi, p in members:
+                g = self._checked(p)
+                rows.append((p.data_ptr(), g.data_ptr(), self._buffer(p, "exp_avg").data_ptr(), self._buffer(p, "exp_avg_sq").data_ptr(),
+                             0, 0.0, p.numel(), gi, 0))
+            self._adopt_steps([p for _, p in members])
+            desc = np.array(rows, dtype=_ADAMW_DTYPE)
+            if self.capturable:
+                desc["step_dev"] = [state[p]["step"].data_ptr() for _, p in members]
+            self._desc["adamw"] = desc
+            self._desc["rows"] = np.array([self._step_of[p] for _, p in members])
+            self._sig["adamw"] = [(p.data_ptr(), p.grad.data_ptr(), state[p]["exp_avg"].data_ptr(), state[p]["exp_avg_sq"].data_ptr(),
+                                   id(state[p]["step"]), gi) for gi, p in members]
+        desc = self._desc["adamw"]
+        if not self.capturable:
+            steps = self._steps.numpy()
+            rows = self._desc["rows"]
+            steps[rows] += 1.0
+            desc["step"] = steps[rows]
+        return desc
+
+    def _adopt_steps(self, params):
+        """state[p]["step"] as views of one flat float tensor (on the host, or on the device for graphs), keeping the values."""
+        device = self._device() if self.capturable else torch.device("cpu")
+        mine = self._step_of if self._step_of is not None else {}
+        if all(p in mine and self.state[p].get("step") is self._views[mine[p]] for p in params):
+            return
+        every = list(dict.fromkeys(list(mine) + list(params)))
+        values = [float(self.state[p]["step"]) if self.state[p].get("step") is not None else 0.0 for p in every]
+        self._steps = torch.tensor(values, dtype=torch.float32, device=device)
+        self._step_of = {p: i for i, p in enumerate(every)}
+        self._views = [self._steps[i] for i in range(len(every))]
+        for p, i in self._step_of.items():
+            self.state[p]["step"] = self._views[i]
+
+    def _refuse_rebuild_in_capture(self):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("%s: a parameter, gradient or state buffer is new while a hipGraph is being captured.  Keep gradients persistent "
+                               "(segmi.distributed.DistributedModel does) and run at least one eager step before capturing." % self._name())
+
+    def _hyper_values(self):
+        raise NotImplementedError
+
+    def push_hyper(self):
+        """Stream-ordered refresh of the device-resident hyper-parameters from `param_groups` (capturable=True only): eager steps do it
+        by themselves, a captured step needs it before each replay."""
+        if not self.capturable:
+            return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("%s.push_hyper must stay outside the captured region (call it before graph replay)" % self._name())
+        values = np.concatenate([v.reshape(-1).view(np.uint8) for v in self._hyper_values()])
+        with torch.cuda.device(self._device()):
+            if self._hyper is None:
+                self._hyper = _Hyper(values.size, self._device())
+            self._hyper.push(values)
+
+    def _ready(self):
+        if torch.cuda.is_current_stream_capturing():
+            if not self.capturable:
+                raise RuntimeError("%s: a step inside a hipGraph capture needs capturable=True (learning rates and step numbers would be "
+                                   "frozen)" % self._name())
+            if self._hyper is None:
+                raise RuntimeError("%s(capturable=True): run one eager step before capturing" % self._name())
+        else:
+            self.push_hyper()
+
+    def _adamw_hyper(self, betas, eps, lr_ratio):
+        h = np.zeros((_MAX_GROUPS, _ADAMW_HYPER), dtype=np.float64)
+        for i, g in enumerate(self.param_groups):
+            h[i] = (float(g["lr"]), float(g["weight_decay"]), float(g[betas][0]), float(g[betas][1]), float(g[eps]))
+            if lr_ratio is not None:
+                h[i, 0] *= float(g[lr_ratio])
+        return h
+
+    def _adamw_launch(self, members, hyper, hyper_dev):
+        desc = self._adamw_descriptors(members)
+        ng, n = len(self.param_groups), len(desc)
+        ws = torch.empty(8 * n, dtype=torch.uint8, device=self._device()) if self.capturable else None
+        check(lib.segmi_adamw_step(desc.ctypes.data, n, hyper.ctypes.data, ng, hyper_dev, None if ws is None else ws.data_ptr(),
+                                   0 if ws is None else 8 * n, torch.cuda.current_stream().cuda_stream), "adamw_step")
+
+    def _live(self):
+        return [(gi, p) for gi, g in enumerate(self.param_groups) for p in g["params"] if p.grad is not None and p.numel()]
+
+
+def _check_common(name, lr, weight_decay, betas, eps):
+    if not float(lr) >= 0.0:
+        raise ValueError("%s: invalid learning rate %r" % (name, lr))
+    if not float(weight_decay) >= 0.0:
+        raise ValueError("%s: invalid weight_decay %r" % (name, weight_decay))
+    if len(betas) != 2 or not all(0.0 <= float(b) < 1.0 for b in betas):
+        raise ValueError("%s: betas must be two numbers in [0, 1), got %r" % (name, betas))
+    if not float(eps) >= 0.0:
+        raise ValueError("%s: invalid eps %r" % (name, eps))
+
+
+class FusedAdamW(_FusedOptimizer):
+    """AdamW (decoupled weight decay) with torch.optim.AdamW's formula, arguments and state layout (`step`, `exp_avg`, `exp_avg_sq`), every
+    parameter in a launch per 56 tensors.  Parameters are float32 CUDA tensors, dense in any memory order.  capturable=True keeps the
+    hyper-parameters and step numbers on the device, for a step captured into a hipGraph (`push_hyper()` before each replay)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, capturable=False):
+        _check_common("segmi.optim.FusedAdamW", lr, weight_decay, betas, eps)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay), capturable)
+
+    def _hyper_values(self):
+        return [self._adamw_hyper("betas", "eps", None)]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        members = self._live()
+        if members:
+            with torch.cuda.device(self._device()):
+                self._ready()
+                self._adamw_launch(members, self._hyper_values()[0], self._hyper.dev.data_ptr() if self.capturable else None)
+        return loss
+
+
+def _matrix_of(p):
+    """(rows, cols) of the dense matrix in p's memory, or None where p is no matrix: vectors, single rows or columns, depthwise filters
+    [C, 1, R, S].  shape[0] x rest, or its transpose where shape[0] runs fastest: the two are orthogonalised alike."""
+    if p.dim() < 2 or (p.dim() == 4 and p.shape[1] == 1):
+        return None
+    r = p.shape[0]
+    c = p.numel() // r if r else 0
+    if min(r, c) < 2:
+        return None
+    if p.stride(0) == c:
+        return r, c
+    if p.stride(0) == 1:
+        return c, r
+    raise RuntimeError("segmi.optim.Muon: a matrix parameter must have its first dimension outermost or innermost in memory, got shape %s "
+                       "strides %s" % (tuple(p.shape), tuple(p.stride())))
+
+
+class Muon(_FusedOptimizer):
+    """Momentum orthogonalised by Newton-Schulz products, for every parameter that is a matrix:
+
+        B <- momentum B + grad;   U = grad + momentum B (nesterov) or B
+        p <- (1 - lr weight_decay) p - lr f orthogonalize(U)
+
+    f = sqrt(max(1, rows / cols)) (adjust_lr_fn None or "original") or 0.2 sqrt(max(rows, cols)) ("match_rms_adamw": updates as
+    large as AdamW's, so one learning rate suits both halves), rows = shape[0].  Argument names follow torch.optim.Muon, which takes 2-D parameters
+    only; this one takes a whole network: vectors, single rows and columns, depthwise filters and the parameters of groups
+    with `"algorithm": "adamw"` are updated by AdamW with learning rate lr * adamw_lr_ratio, adamw_betas, adamw_eps and the group's weight_decay.
+    State: `momentum_buffer`, or `step`, `exp_avg`, `exp_avg_sq`.  Learning rate, weight decay, momentum and the AdamW
+    numbers may differ between groups (up to 8); nesterov, eps, ns_coefficients and ns_steps are one for all.  A parameter without gradient is
+    left alone.  capturable=True: as segmi.optim.SGD."""
+
+    _SHARED = ("nesterov", "eps", "ns_coefficients", "ns_steps")
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=NS_COEFFICIENTS, eps=1e-7, ns_steps=5,
+                 adjust_lr_fn=None, adamw_lr_ratio=1.0, adamw_betas=(0.9, 0.95), adamw_eps=1e-8, capturable=False):
+        _check_common("segmi.optim.Muon", lr, weight_decay, adamw_betas, adamw_eps)
+        if not 0.0 <= float(momentum) < 1.0:
+            raise ValueError("segmi.optim.Muon: momentum must be in [0, 1), got %r" % (momentum,))
+        if not float(adamw_lr_ratio) >= 0.0:
+            raise ValueError("segmi.optim.Muon: invalid adamw_lr_ratio %r" % (adamw_lr_ratio,))
+        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
+            raise ValueError("segmi.optim.Muon: adjust_lr_fn must be None, 'original' or 'match_rms_adamw', got %r" % (adjust_lr_fn,))
+        _check_iteration(ns_steps, ns_coefficients, eps, "segmi.optim.Muon")
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=bool(nesterov),
+                                      ns_coefficients=tuple(ns_coefficients), eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn,
+                                      adamw_lr_ratio=adamw_lr_ratio, adamw_betas=tuple(adamw_betas), adamw_eps=adamw_eps, algorithm="auto"),
+                         capturable)
+
+    def add_param_group(self, group):
+        if group.get("algorithm", "auto") not in ("auto", "adamw"):
+            raise ValueError("segmi.optim.Muon: a group's algorithm is 'auto' or 'adamw', got %r" % (group["algorithm"],))
+        super().add_param_group(group)
+
+    def _hyper_values(self):
+        h = np.zeros((3, _MAX_GROUPS), dtype=np.float32)
+        for i, g in enumerate(self.param_groups):
+            h[:, i] = float(g["lr"]), float(g["weight_decay"]), float(g["momentum"])
+        return [h, self._adamw_hyper("adamw_betas", "adamw_eps", "adamw_lr_ratio")]
+
+    def _muon_descriptors(self, members):
+        state = self.state
+        sig = [(p.data_ptr(), p.grad.data_ptr(), b.data_ptr() if b is not None else 0, gi, self.param_groups[gi]["adjust_lr_fn"])
+               for gi, p in members for b in (state[p].get("momentum_buffer"),)]
+        if sig != self._sig.get("muon"):
+            self._refuse_rebuild_in_capture()
+            rows = []
+            for gi, p in members:
+                g, (r, c) = self._checked(p), _matrix_of(p)
+                k, rest = p.shape[0], p.numel() // p.shape[0]
+                if self.param_groups[gi]["adjust_lr_fn"] == "match_rms_adamw":
+                    f = 0.2 * math.sqrt(max(k, rest))
+                else:
+                    f = math.sqrt(max(1.0, k / rest))
+                rows.append((p.data_ptr(), g.data_ptr(), self._buffer(p, "momentum_buffer").data_ptr(), r, c, f, gi))
+            desc = self._desc["muon"] = np.array(rows, dtype=_MUON_DTYPE)
+            self._desc["bytes"] = lib.segmi_muon_workspace(desc.ctypes.data, len(desc))
+            if not self._desc["bytes"]:
+                raise SegmiError("segmi.optim.Muon: a matrix is too large (4 GiB of float32 after padding its sides to 64)")
+            self._sig["muon"] = [(p.data_ptr(), p.grad.data_ptr(), state[p]["momentum_buffer"].data_ptr(), gi, self.param_groups[gi]["adjust_lr_fn"])
+                                 for gi, p in members]
+        return self._desc["muon"]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        groups = self.param_groups
+        first = groups[0]
+        for g in groups[1:]:
+            if any(g[k] != first[k] for k in self._SHARED):
+                raise ValueError("segmi.optim.Muon: %s must be the same in all parameter groups" % ", ".join(self._SHARED))
+        mats, rest = [], []
+        for gi, p in self._live():
+            is_matrix = groups[gi].get("algorithm", "auto") == "auto" and _matrix_of(p) is not None
+            (mats if is_matrix else rest).append((gi, p))
+        if not mats and not rest:
+            return loss
+        coef = _check_iteration(first["ns_steps"], first["ns_coefficients"], first["eps"], "segmi.optim.Muon")
+        with torch.cuda.device(self._device()):
+            self._ready()
+            hd = self._hyper.dev.data_ptr() if self.capturable else None
+            h, a = self._hyper_values()
+            ng = len(groups)
+            if mats:
+                desc = self._muon_descriptors(mats)
+                nbytes = self._desc["bytes"]
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=self._device())
+                check(lib.segmi_muon_step(desc.ctypes.data, len(desc), h[0].ctypes.data, h[1].ctypes.data, h[2].ctypes.data, ng, hd,
+                                          1 if first["nesterov"] else 0, coef, int(first["ns_steps"]), float(first["eps"]), ws.data_ptr(), nbytes,
+                                          torch.cuda.current_stream().cuda_stream), "muon_step")
+            if rest:
+                self._adamw_launch(rest, a, hd + 4 * 3 * _MAX_GROUPS if hd else None)
+        return loss

@@ -15,6 +15,7 @@ import numpy as np
 import torch
 
 from ._lib import check, lib
+from .muon import FusedAdamW, Muon, orthogonalize  # noqa: F401  (public here: segmi.optim.Muon, ...; defined in muon.py)
 
 
 class _Chunk(C.Structure):
