@@ -6,10 +6,12 @@
 // polynomials of A, so X_L = (Q_{L-1} ... Q_0) X_0 with A_{k+1} = Q_k A_k Q_k, and a segment of L steps reads the large matrix twice
 // (its Gram product and the product with P = Q_{L-1} ... Q_0) instead of 2 L times.  Rounding in A_k acts on the SQUARES of
 // the singular values and is amplified by a^2 a step, so X is formed and its Gram matrix taken anew after segments of 2 and 1 steps.
-// Median distance from 64-bit results relative to the fp32 iteration's (64 x 128 noise with strong directions / 256 x 512 low rank):
-// five steps as 2 + 1 + 2: 1.06 / 1.5, one by one: 1.05 / 2.3, 1 + 2 + 2: 2.3 / 2.1, 3 + 2: 6.1 / 1.2.  Of these 2 + 1 + 2 needs
-// 9 m^2 n + 11 m^3 operations, one by one 15 m^2 n + 5 m^3 (both with symmetric products halved): the same for square matrices, fewer for
-// all others.
+// A segment of one step leaves the identity out of the product, X <- a X + (b A + c A^2) X: the part that carries small
+// singular values is then not rounded through a matrix whose entries are as large as a.  Median distance from 64-bit results relative to the
+// fp32 iteration's, noise with strong directions 128 x 128 / 64 x 128, low rank 256 x 512: five steps as 2 + 1 + 2: 1.8 / 1.06 /
+// 1.5, one by one: 1.07 / 1.05 / 1.1, 1 + 2 + 2: 2.4 / 2.3 / 2.1, 3 + 2: 3.6 / 6.1 / 1.2.  One by one needs 15 m^2 n + 5 m^3 operations
+// (symmetric products halved), 2 + 1 + 2 9 m^2 n + 11 m^3: the same for square matrices, which therefore go one by one up to
+// n < 2 m, and fewer the wider they are.
 //
 // Arithmetic.  Every matrix is held as hi + lo, two fp16 numbers of one value scaled by a power of two (22 - 23 significant bits; fp32
 // has 24), and a product is hi hi + hi lo + lo hi on v_mfma_f32_32x32x16_f16 with fp32 accumulators.  The dropped lo lo term and the
@@ -283,6 +285,7 @@ struct Tile {
     static constexpr unsigned STAGE = 2 * BT * LINE;
     f32x16 acc[S][S];
 
+    // The two mixed products have an accumulator of their own, added at the end: the large sum is rounded a third as often.
     __device__ __forceinline__ void run(char* smem, const char* L, unsigned rows_l, const char* R, unsigned rows_r, unsigned lines,
                                         unsigned l0, unsigned r0, unsigned q0, unsigned q1) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -299,12 +302,13 @@ struct Tile {
             off_l[p] = (l0 + row) * pitch + chunk * 16;
             off_r[p] = (r0 + row) * pitch + chunk * 16;
         }
+        f32x16 mix[S][S];
 #pragma unroll
         for (int i = 0; i < S; ++i)
 #pragma unroll
             for (int j = 0; j < S; ++j)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.f;
+                for (int x = 0; x < 16; ++x) acc[i][j][x] = mix[i][j][x] = 0.f;
 
         auto issue = [&](unsigned q, unsigned stage) {
 #pragma unroll
@@ -339,11 +343,11 @@ struct Tile {
 #pragma unroll
                 for (int i = 0; i < S; ++i)
 #pragma unroll
-                    for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll[i], rh[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < S; ++j) mix[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll[i], rh[j], mix[i][j], 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < S; ++i)
 #pragma unroll
-                    for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[i], rl8[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < S; ++j) mix[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[i], rl8[j], mix[i][j], 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < S; ++i)
 #pragma unroll
@@ -352,6 +356,12 @@ struct Tile {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
         }
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) acc[i][j][x] += mix[i][j][x];
     }
 
     // f(i, j, g, row, col): values acc[i][j][4 g .. 4 g + 3] are rows row .. row+3 of column col (tile-relative)
@@ -393,16 +403,12 @@ struct Product {
     float scale;                     // fp32 sum -> stored result
     float ident, lin;                // out = ident I + lin A + scale L R^T (POLY only; A in its stored scale)
 };
-struct ProductPair {
-    Product p[2];
-};
 
-// m x m products (all operands symmetric): A^2 with the polynomial's epilogue, Q A, W Q, P Q.  Two independent ones share a launch.
+// m x m products (all operands symmetric): A^2 with the polynomial's epilogue, Q A, W Q, P Q.
 template <int BT, bool POLY>
-__global__ __launch_bounds__(256, 2) void ns_square_product(Batch b, ProductPair pp) {
+__global__ __launch_bounds__(256, 2) void ns_square_product(Batch b, Product pr) {
     __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<BT>::STAGE];
     const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
-    const Product pr = pp.p[blockIdx.y];
     const Item s = b.item[find_item(b, wg)];
     char* const base = b.ws + (size_t)s.base * 256;
     const unsigned M = pad64(s.m), lines = M / 32;
@@ -506,9 +512,10 @@ __global__ __launch_bounds__(256) void ns_gram_reduce(GramBatch b) {
     store_symmetric(b.ws + (size_t)s.base * 256 + buffer_offset(A, s.m, s.n), M / 32, row, col, r4, ti != tj);
 }
 
-// X <- P X between segments: both orders again (T1 from T0, X in place: no workgroup reads X)
+// X <- alpha X + P X between segments (alpha = 0 where P holds the identity's part): both orders again (T1 from T0, X in place:
+// no workgroup reads X)
 template <int BT>
-__global__ __launch_bounds__(256, 2) void ns_apply(Batch b, int p, int tin, int tout, float scale) {
+__global__ __launch_bounds__(256, 2) void ns_apply(Batch b, int p, int tin, int tout, float scale, float alpha) {
     __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<BT>::STAGE];
     const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
     const Item s = b.item[find_item(b, wg)];
@@ -519,12 +526,19 @@ __global__ __launch_bounds__(256, 2) void ns_apply(Batch b, int p, int tin, int 
     t.run(smem, base + buffer_offset(p, s.m, s.n), M, base + buffer_offset(tin, s.m, s.n), N, M / 32, ti * BT, tj * BT, 0, M / 32);
     char* const xo = base;
     char* const to = base + buffer_offset(tout, s.m, s.n);
+    const char* const ti4 = base + buffer_offset(tin, s.m, s.n);
     t.each4([&](int row, int col, const float* acc) {
         const unsigned r = ti * BT + row, c = tj * BT + col;
         if (r >= M || c >= N) return;
         float v[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) v[x] = acc[x] * scale;
+        if (alpha != 0.f) {
+            float old[4];
+            load4(ti4, M / 32, c, r, old);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = fmaf(alpha, old[x], v[x]);
+        }
         store4(to, M / 32, c, r, v);
 #pragma unroll
         for (int x = 0; x < 4; ++x) store1(xo, N / 32, r + x, c, v[x]);
@@ -545,7 +559,7 @@ struct TargetBatch {
     char* ws;
     int count;
     int p, tin;
-    float scale;
+    float scale, alpha;              // of the stored sum, of the stored X (as in ns_apply)
     Target item[BATCH];
 };
 
@@ -570,23 +584,28 @@ __global__ __launch_bounds__(256, 2) void ns_finish(TargetBatch b, Hyper h, cons
     if (MUON) {
         const float lr = hd ? hd->lr[s.group] : h.lr[s.group], wd = hd ? hd->wd[s.group] : h.wd[s.group];
         keep = 1.f - lr * wd;
-        step = lr * s.factor * b.scale;
+        step = lr * s.factor;
     }
+    const char* const old = s.turned ? base : T;         // row c of it, values r .. r+3: X's own order, or the other one
+    const unsigned old_lines = (s.turned ? N : M) / 32;
     t.each4([&](int row, int col, const float* acc) {
         const unsigned c = c0 + col;
-        if (c >= cols) return;
+        if (c >= cols || r0 + row >= rows) return;
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+        if (b.alpha != 0.f) load4(old, old_lines, c, r0 + row, o);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const unsigned r = r0 + row + x;
             if (r >= rows) break;
+            const float v = fmaf(b.alpha, o[x], acc[x] * b.scale);
             const long at = (long)r * sr + (long)c * sc;
             if (MUON) {
                 float* const p = static_cast<float*>(s.dst) + at;
-                *p = fmaf(-step, acc[x], *p * keep);
+                *p = fmaf(-step, v, *p * keep);
             } else if (s.dtype) {
-                static_cast<unsigned short*>(s.dst)[at] = f32_to_bf16(acc[x] * b.scale);
+                static_cast<unsigned short*>(s.dst)[at] = f32_to_bf16(v);
             } else {
-                static_cast<float*>(s.dst)[at] = acc[x] * b.scale;
+                static_cast<float*>(s.dst)[at] = v;
             }
         }
     });
@@ -604,6 +623,15 @@ struct Bounds {
     }
     double p(double s) const { return std::fabs(s * (a + s * s * (b + s * s * c))); }
     double q(double s) const { return std::fabs(a + s * s * (b + s * s * c)); }
+    double r(double s) const { return std::fabs(s * s * (b + s * s * c)); }
+    double max_r(double s) const {
+        double v = std::fmax(r(s), 1e-6);
+        if (c != 0.0) {
+            const double y = -b / (2.0 * c);
+            if (y > 0.0 && y < s * s) v = std::fmax(v, r(std::sqrt(y)));
+        }
+        return v;
+    }
     double max_p(double s) const {
         double v = p(s);
         // p' = a + 3 b y + 5 c y^2, y = s^2
@@ -634,15 +662,17 @@ struct Bounds {
 constexpr double SLACK = 1.0 + 1e-5;                     // what rounding may add to a bound
 constexpr double MAX_BOUND = 4096.0;                     // coefficients whose iterates grow beyond this are refused
 
-// 2, 1, 2, 1, ... steps between Gram products, see the head of this file
-int segment_length(int index, int left) { return (index & 1) == 0 && left >= 2 ? 2 : 1; }
+// Steps between Gram products: one by one for matrices of nearly square shape, else 2, 1, 2, 1, ... (see the head of this file)
+int segment_length(bool wide, int index, int left) { return wide && (index & 1) == 0 && left >= 2 ? 2 : 1; }
+bool is_wide(int rows, int cols) { return rows <= cols ? cols / 2 >= rows : rows / 2 >= cols; }
 
 bool iteration_ok(const Bounds& f, int steps) {
     double s = SLACK;
     for (int left = steps, seg = 0; left > 0; ++seg) {
         double P = 1.0;
-        for (int i = segment_length(seg, left); i > 0; --i, --left) {
+        for (int i = segment_length(true, seg, left); i > 0; --i, --left) {
             P *= f.max_q(s) * SLACK;
+            if (!(f.max_r(s) < MAX_BOUND)) return false;
             s = f.max_p(s) * SLACK;
             if (!(P > 1e-6 && P < MAX_BOUND && s > 1e-6 && s < MAX_BOUND)) return false;
         }
@@ -742,56 +772,53 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
     src.scale = (float)sx;
     hipLaunchKernelGGL((ns_normalise<MUON>), dim3(g_norm), dim3(256), 0, st, src, h, hd);
 
+    const bool wide = is_wide(shapes[0].m, shapes[0].n);
     int tin = T0;
     for (int left = steps, seg = 0; left > 0; ++seg) {
-        const int len = segment_length(seg, left);
+        const int len = segment_length(wide, seg, left);
         double sa = Bounds::scale_for(s * s);
         gram.scale = (float)(sa / (sx * sx));
         hipLaunchKernelGGL((ns_gram<BT>), dim3(g_gram), dim3(256), 0, st, gram);
         hipLaunchKernelGGL((ns_gram_reduce<BT>), dim3(g_red), dim3(256), 0, st, gram);
+        const auto product = [&](int l, int r, int out, double so, double sl, double sr) { return Product{l, r, out, (float)(so / (sl * sr)), 0.f, 0.f}; };
+        const auto square = [&](int out, double so, double ident) {      // out = ident I + b A + c A^2
+            const Product pr{A, A, out, (float)(f.c * so / (sa * sa)), (float)(ident * so), (float)(f.b * so / sa)};
+            hipLaunchKernelGGL((ns_square_product<BT, true>), dim3(g_sq), dim3(256), 0, st, sq, pr);
+        };
+        const double s1 = f.max_p(s) * SLACK;            // bound after the segment's first step
+        double sp, alpha = 0.0;
         int p = P0;
-        double bp = 1.0, sp = 1.0;
-        for (int i = 0; i < len; ++i) {
-            const double bq = f.max_q(s) * SLACK, bnext = f.max_p(s) * SLACK, bw = s * bnext;
-            const double sqs = Bounds::scale_for(bq);
-            const int qbuf = i == 0 ? P0 : Q;            // the first Q of a segment is its P
-            ProductPair pp;
-            pp.p[0] = Product{A, A, qbuf, (float)(f.c * sqs / (sa * sa)), (float)(f.a * sqs), (float)(f.b * sqs / sa)};
-            pp.p[1] = pp.p[0];
-            hipLaunchKernelGGL((ns_square_product<BT, true>), dim3(g_sq), dim3(256), 0, st, sq, pp);
-            int two = 0;
-            if (i == 0) {
-                bp = bq;
-                sp = sqs;
-            } else {
-                const double nsp = Bounds::scale_for(bp * bq);
-                const int np = p == P0 ? P1 : P0;
-                pp.p[two++] = Product{p, Q, np, (float)(nsp / (sp * sqs)), 0.f, 0.f};
-                bp *= bq;
-                sp = nsp;
-                p = np;
-            }
-            const double sw = Bounds::scale_for(bw), san = Bounds::scale_for(bnext * bnext);
-            if (i + 1 < len) pp.p[two++] = Product{qbuf, A, W, (float)(sw / (sqs * sa)), 0.f, 0.f};
-            if (two) hipLaunchKernelGGL((ns_square_product<BT, false>), dim3(g_sq, two), dim3(256), 0, st, sq, pp);
-            if (i + 1 < len) {
-                pp.p[0] = Product{W, qbuf, A, (float)(san / (sw * sqs)), 0.f, 0.f};
-                hipLaunchKernelGGL((ns_square_product<BT, false>), dim3(g_sq), dim3(256), 0, st, sq, pp);
-                sa = san;
-            }
-            s = bnext;
+        if (len == 1) {
+            sp = Bounds::scale_for(f.max_r(s) * SLACK);
+            square(P0, sp, 0.0);
+            alpha = f.a;
+            s = s1;
+        } else {
+            // P0 = Q(A), W = P0 A, A <- W P0, Q = Q(A), P1 = P0 Q
+            const double bq0 = f.max_q(s) * SLACK, bq1 = f.max_q(s1) * SLACK;
+            const double sq0 = Bounds::scale_for(bq0), sw = Bounds::scale_for(s * s1), san = Bounds::scale_for(s1 * s1), sq1 = Bounds::scale_for(bq1);
+            square(P0, sq0, f.a);
+            hipLaunchKernelGGL((ns_square_product<BT, false>), dim3(g_sq), dim3(256), 0, st, sq, product(P0, A, W, sw, sq0, sa));
+            hipLaunchKernelGGL((ns_square_product<BT, false>), dim3(g_sq), dim3(256), 0, st, sq, product(W, P0, A, san, sw, sq0));
+            sa = san;
+            square(Q, sq1, f.a);
+            sp = Bounds::scale_for(bq0 * bq1);
+            hipLaunchKernelGGL((ns_square_product<BT, false>), dim3(g_sq), dim3(256), 0, st, sq, product(P0, Q, P1, sp, sq0, sq1));
+            p = P1;
+            s = f.max_p(s1) * SLACK;
         }
         left -= len;
         if (left > 0) {
             const double nsx = Bounds::scale_for(s);
             const int tout = tin == T0 ? T1 : T0;
-            hipLaunchKernelGGL((ns_apply<BT>), dim3(g_big), dim3(256), 0, st, big, p, tin, tout, (float)(nsx / (sp * sx)));
+            hipLaunchKernelGGL((ns_apply<BT>), dim3(g_big), dim3(256), 0, st, big, p, tin, tout, (float)(nsx / (sp * sx)), (float)(alpha * nsx / sx));
             tin = tout;
             sx = nsx;
         } else {
             dst.p = p;
             dst.tin = tin;
             dst.scale = (float)(1.0 / (sp * sx));
+            dst.alpha = (float)(alpha / sx);
             hipLaunchKernelGGL((ns_finish<BT, MUON>), dim3(g_big), dim3(256), 0, st, dst, h, hd);
         }
     }
@@ -809,17 +836,34 @@ Shape shape_of(int rows, int cols, bool cols_inner) {
 
 Shape shape_of(const segmi_ns_matrix& a) { return shape_of(a.rows, a.cols, a.src_cs == 1 || a.src_rs != 1); }
 
-// workspace of a call: its batches run one after the other and share it
+// The matrices of a call in batches of one class (wide or not) and at most BATCH each: f(indices, how many) in order, until it
+// returns something other than SEGMI_OK.  Batches run one after the other and share the workspace.
+template <typename M, typename F>
+int for_batches(const M* mats, int count, F f) {
+    for (int wide = 0; wide < 2; ++wide) {
+        int index[BATCH], k = 0;
+        for (int i = 0; i < count; ++i) {
+            if (is_wide(mats[i].rows, mats[i].cols) == (wide != 0)) index[k++] = i;
+            if (k == BATCH || (i == count - 1 && k)) {
+                const int rc = f(index, k);
+                if (rc != SEGMI_OK) return rc;
+                k = 0;
+            }
+        }
+    }
+    return SEGMI_OK;
+}
+
 template <typename M, typename F>
 size_t workspace_of(const M* mats, int count, F shape) {
     size_t most = 0;
-    Shape s[BATCH];
-    for (int at = 0; at < count; at += BATCH) {
-        const int k = count - at < BATCH ? count - at : BATCH;
-        for (int i = 0; i < k; ++i) s[i] = shape(mats[at + i]);
+    for_batches(mats, count, [&](const int* index, int k) {
+        Shape s[BATCH];
+        for (int i = 0; i < k; ++i) s[i] = shape(mats[index[i]]);
         const Plan p = plan_batch(s, k);
         if (p.bytes > most) most = p.bytes;
-    }
+        return (int)SEGMI_OK;
+    });
     return most;
 }
 
@@ -849,14 +893,13 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
     if ((size_t)workspace & 255) return SEGMI_ERR_ALIGN;
     if (workspace_bytes < segmi_ns_workspace(mats_host, count)) return SEGMI_ERR_WORKSPACE;
     const Bounds f{coefficients_host[0], coefficients_host[1], coefficients_host[2]};
-    for (int at = 0; at < count; at += BATCH) {
-        const int k = count - at < BATCH ? count - at : BATCH;
+    return for_batches(mats_host, count, [&](const int* index, int k) {
         Shape shapes[BATCH];
         SourceBatch src{};
         TargetBatch dst{};
         src.eps = eps;
         for (int i = 0; i < k; ++i) {
-            const segmi_ns_matrix& a = mats_host[at + i];
+            const segmi_ns_matrix& a = mats_host[index[i]];
             const Shape s = shapes[i] = shape_of(a);
             const bool cols_inner = a.src_cs == 1 || a.src_rs != 1, wide = a.rows <= a.cols;
             Source& o = src.item[i];
@@ -876,10 +919,8 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
             t.dtype = a.dtype;
             t.turned = t.si == 1 && t.sj != 1;
         }
-        const int rc = run_batch<false>(shapes, src, dst, k, f, steps, static_cast<char*>(workspace), Hyper{}, nullptr, (hipStream_t)stream);
-        if (rc != SEGMI_OK) return rc;
-    }
-    return SEGMI_OK;
+        return run_batch<false>(shapes, src, dst, k, f, steps, static_cast<char*>(workspace), Hyper{}, nullptr, (hipStream_t)stream);
+    });
 }
 
 size_t segmi_muon_workspace(const segmi_muon_matrix* mats_host, int count) {
@@ -909,15 +950,14 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
             h.wd[i] = weight_decay_host[i];
             h.mom[i] = momentum_host[i];
         }
-    for (int at = 0; at < count; at += BATCH) {
-        const int k = count - at < BATCH ? count - at : BATCH;
+    return for_batches(mats_host, count, [&](const int* index, int k) {
         Shape shapes[BATCH];
         SourceBatch src{};
         TargetBatch dst{};
         src.eps = eps;
         src.nesterov = nesterov;
         for (int i = 0; i < k; ++i) {
-            const segmi_muon_matrix& a = mats_host[at + i];
+            const segmi_muon_matrix& a = mats_host[index[i]];
             const Shape s = shapes[i] = shape_of(a.rows, a.cols, true);
             const bool wide = a.rows <= a.cols;
             Source& o = src.item[i];
@@ -939,11 +979,9 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
             t.group = a.group;
             t.turned = !wide;
         }
-        const int rc = run_batch<true>(shapes, src, dst, k, f, steps, static_cast<char*>(workspace), h,
-                                       reinterpret_cast<const Hyper*>(hyper_dev), (hipStream_t)stream);
-        if (rc != SEGMI_OK) return rc;
-    }
-    return SEGMI_OK;
+        return run_batch<true>(shapes, src, dst, k, f, steps, static_cast<char*>(workspace), h, reinterpret_cast<const Hyper*>(hyper_dev),
+                               (hipStream_t)stream);
+    });
 }
 
 }  // extern "C"
