@@ -662,9 +662,13 @@ struct Bounds {
 constexpr double SLACK = 1.0 + 1e-5;                     // what rounding may add to a bound
 constexpr double MAX_BOUND = 4096.0;                     // coefficients whose iterates grow beyond this are refused
 
-// Steps between Gram products: one by one for matrices of nearly square shape, else 2, 1, 2, 1, ... (see the head of this file)
+// Steps between Gram products: one by one for matrices of nearly square shape and for small ones, else 2, 1, 2, 1, ... (see the head
+// of this file; below 65 rows the sums are so short that fp32 rounds hardly at all, and 2 + 1 + 2 came out at up to 2.2 times its distance)
 int segment_length(bool wide, int index, int left) { return wide && (index & 1) == 0 && left >= 2 ? 2 : 1; }
-bool is_wide(int rows, int cols) { return rows <= cols ? cols / 2 >= rows : rows / 2 >= cols; }
+bool is_wide(int rows, int cols) {
+    const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+    return m > 64 && n / 2 >= m;
+}
 
 bool iteration_ok(const Bounds& f, int steps) {
     double s = SLACK;
@@ -689,19 +693,39 @@ struct Plan {
     size_t partial_at, gram_at, mats_at, bytes;
 };
 
-constexpr int BT = 64;
+unsigned tiles_of(int m, int bt) { return (pad64(m) + bt - 1) / bt; }
+unsigned low_tiles(int m, int bt) { const unsigned t = tiles_of(m, bt); return t * (t + 1) / 2; }
+unsigned big_tiles(const Shape& s, int bt) { return tiles_of(s.m, bt) * tiles_of(s.n, bt); }
 
-unsigned tiles_of(int m) { return pad64(m) / BT; }
+// Tile size of a launch: 128 x 128 where that still gives every CU a workgroup
+template <typename F>
+int tile_size(const Shape* s, int count, F tiles) {
+    size_t t = 0;
+    for (int i = 0; i < count; ++i) t += tiles(s[i], 128);
+    return t >= SEGMI_NUM_CU ? 128 : 64;
+}
+#define NS_LAUNCH(bt, kernel128, kernel64, grid, ...)                                                          \
+    do {                                                                                                       \
+        if ((bt) == 128) hipLaunchKernelGGL(kernel128, dim3(grid), dim3(256), 0, st, __VA_ARGS__);             \
+        else hipLaunchKernelGGL(kernel64, dim3(grid), dim3(256), 0, st, __VA_ARGS__);                          \
+    } while (0)
 
 // runs of a Gram product: enough workgroups to fill the chip, no run shorter than 8 lines
-unsigned gram_run(const Shape* s, int count) {
-    double work = 0.0;
+struct GramPlan {
+    int bt;
+    unsigned run;
+};
+GramPlan gram_plan(const Shape* s, int count) {
+    GramPlan best{64, 0};
+    double work128 = 0.0, work64 = 0.0;
     for (int i = 0; i < count; ++i) {
-        const unsigned t = tiles_of(s[i].m);
-        work += (double)(t * (t + 1) / 2) * (pad64(s[i].n) / 32);
+        work128 += (double)low_tiles(s[i].m, 128) * (pad64(s[i].n) / 32);
+        work64 += (double)low_tiles(s[i].m, 64) * (pad64(s[i].n) / 32);
     }
-    const double run = std::ceil(work / 2048.0);
-    return run < 8.0 ? 8u : (unsigned)run;
+    best.bt = work128 / 8.0 >= 512.0 ? 128 : 64;
+    const double run = std::ceil((best.bt == 128 ? work128 / 1024.0 : work64 / 2048.0));
+    best.run = run < 8.0 ? 8u : (unsigned)run;
+    return best;
 }
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -709,16 +733,16 @@ size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 Plan plan_batch(const Shape* s, int count) {
     Plan p;
     size_t parts = 0, slots = 0, mats = 0;
-    const unsigned run = gram_run(s, count);
+    const GramPlan g = gram_plan(s, count);
     for (int i = 0; i < count; ++i) {
-        const unsigned t = tiles_of(s[i].m), lines = pad64(s[i].n) / 32;
+        const unsigned lines = pad64(s[i].n) / 32;
         parts += (size_t)segmi_cdiv(s[i].outer, 64) * segmi_cdiv(s[i].inner, 256);
-        slots += (size_t)(t * (t + 1) / 2) * segmi_cdiv(lines, run);
+        slots += (size_t)low_tiles(s[i].m, g.bt) * segmi_cdiv(lines, g.run);
         mats += 3 * big_bytes(s[i].m, s[i].n) + 5 * square_bytes(s[i].m);
     }
     p.partial_at = 0;
     p.gram_at = align256(parts * sizeof(double));
-    p.mats_at = p.gram_at + align256(slots * BT * BT * sizeof(float));
+    p.mats_at = p.gram_at + align256(slots * g.bt * g.bt * sizeof(float));
     p.bytes = p.mats_at + mats;
     return p;
 }
@@ -728,7 +752,9 @@ template <bool MUON>
 int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count, const Bounds& f, int steps, char* ws,
               const Hyper& h, const Hyper* hd, hipStream_t st) {
     const Plan plan = plan_batch(shapes, count);
-    const unsigned run = gram_run(shapes, count);
+    const GramPlan gp = gram_plan(shapes, count);
+    const int bt_sq = tile_size(shapes, count, [](const Shape& x, int bt) { return low_tiles(x.m, bt); });
+    const int bt_big = tile_size(shapes, count, big_tiles);
     Batch sq, big;
     GramBatch gram;
     src.ws = dst.ws = sq.ws = big.ws = gram.ws = ws + plan.mats_at;
@@ -740,7 +766,7 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
     size_t base = 0;
     for (int i = 0; i < count; ++i) {
         const Shape& s = shapes[i];
-        const unsigned t = tiles_of(s.m), lines = pad64(s.n) / 32, low = t * (t + 1) / 2, splits = segmi_cdiv(lines, run);
+        const unsigned lines = pad64(s.n) / 32, low = low_tiles(s.m, gp.bt), splits = segmi_cdiv(lines, gp.run);
         const unsigned b256 = (unsigned)(base / 256);
         const unsigned units = segmi_cdiv(s.outer, 64) * segmi_cdiv(s.inner, 256);
         src.item[i].base = dst.item[i].base = b256;
@@ -748,17 +774,17 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
         src.item[i].part = parts;
         src.item[i].parts = units;
         sq.item[i] = Item{g_sq, s.m, s.n, b256};
-        gram.item[i] = GramItem{g_gram, slots, s.m, s.n, b256, low, splits, run};
+        gram.item[i] = GramItem{g_gram, slots, s.m, s.n, b256, low, splits, gp.run};
         big.item[i] = Item{g_big, s.m, s.n, b256};
         dst.item[i].first = g_big;
         g_sum += units;
         parts += units;
         g_norm += (pad64(s.outer) / 64) * (pad64(s.inner) / 64);
-        g_sq += low;
+        g_sq += low_tiles(s.m, bt_sq);
         g_gram += low * splits;
-        g_red += low * (BT / 32) * (BT / 32);
+        g_red += low * (gp.bt / 32) * (gp.bt / 32);
         slots += low * splits;
-        g_big += t * (pad64(s.n) / BT);
+        g_big += big_tiles(s, bt_big);
         base += 3 * big_bytes(s.m, s.n) + 5 * square_bytes(s.m);
     }
     hipLaunchKernelGGL((ns_sum_squares<MUON>), dim3(g_sum), dim3(256), 0, st, src, h, hd);
@@ -778,12 +804,12 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
         const int len = segment_length(wide, seg, left);
         double sa = Bounds::scale_for(s * s);
         gram.scale = (float)(sa / (sx * sx));
-        hipLaunchKernelGGL((ns_gram<BT>), dim3(g_gram), dim3(256), 0, st, gram);
-        hipLaunchKernelGGL((ns_gram_reduce<BT>), dim3(g_red), dim3(256), 0, st, gram);
+        NS_LAUNCH(gp.bt, ns_gram<128>, ns_gram<64>, g_gram, gram);
+        NS_LAUNCH(gp.bt, ns_gram_reduce<128>, ns_gram_reduce<64>, g_red, gram);
         const auto product = [&](int l, int r, int out, double so, double sl, double sr) { return Product{l, r, out, (float)(so / (sl * sr)), 0.f, 0.f}; };
         const auto square = [&](int out, double so, double ident) {      // out = ident I + b A + c A^2
             const Product pr{A, A, out, (float)(f.c * so / (sa * sa)), (float)(ident * so), (float)(f.b * so / sa)};
-            hipLaunchKernelGGL((ns_square_product<BT, true>), dim3(g_sq), dim3(256), 0, st, sq, pr);
+            NS_LAUNCH(bt_sq, (ns_square_product<128, true>), (ns_square_product<64, true>), g_sq, sq, pr);
         };
         const double s1 = f.max_p(s) * SLACK;            // bound after the segment's first step
         double sp, alpha = 0.0;
@@ -798,12 +824,12 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
             const double bq0 = f.max_q(s) * SLACK, bq1 = f.max_q(s1) * SLACK;
             const double sq0 = Bounds::scale_for(bq0), sw = Bounds::scale_for(s * s1), san = Bounds::scale_for(s1 * s1), sq1 = Bounds::scale_for(bq1);
             square(P0, sq0, f.a);
-            hipLaunchKernelGGL((ns_square_product<BT, false>), dim3(g_sq), dim3(256), 0, st, sq, product(P0, A, W, sw, sq0, sa));
-            hipLaunchKernelGGL((ns_square_product<BT, false>), dim3(g_sq), dim3(256), 0, st, sq, product(W, P0, A, san, sw, sq0));
+            NS_LAUNCH(bt_sq, (ns_square_product<128, false>), (ns_square_product<64, false>), g_sq, sq, product(P0, A, W, sw, sq0, sa));
+            NS_LAUNCH(bt_sq, (ns_square_product<128, false>), (ns_square_product<64, false>), g_sq, sq, product(W, P0, A, san, sw, sq0));
             sa = san;
             square(Q, sq1, f.a);
             sp = Bounds::scale_for(bq0 * bq1);
-            hipLaunchKernelGGL((ns_square_product<BT, false>), dim3(g_sq), dim3(256), 0, st, sq, product(P0, Q, P1, sp, sq0, sq1));
+            NS_LAUNCH(bt_sq, (ns_square_product<128, false>), (ns_square_product<64, false>), g_sq, sq, product(P0, Q, P1, sp, sq0, sq1));
             p = P1;
             s = f.max_p(s1) * SLACK;
         }
@@ -811,7 +837,7 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
         if (left > 0) {
             const double nsx = Bounds::scale_for(s);
             const int tout = tin == T0 ? T1 : T0;
-            hipLaunchKernelGGL((ns_apply<BT>), dim3(g_big), dim3(256), 0, st, big, p, tin, tout, (float)(nsx / (sp * sx)), (float)(alpha * nsx / sx));
+            NS_LAUNCH(bt_big, ns_apply<128>, ns_apply<64>, g_big, big, p, tin, tout, (float)(nsx / (sp * sx)), (float)(alpha * nsx / sx));
             tin = tout;
             sx = nsx;
         } else {
@@ -819,7 +845,7 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
             dst.tin = tin;
             dst.scale = (float)(1.0 / (sp * sx));
             dst.alpha = (float)(alpha / sx);
-            hipLaunchKernelGGL((ns_finish<BT, MUON>), dim3(g_big), dim3(256), 0, st, dst, h, hd);
+            NS_LAUNCH(bt_big, (ns_finish<128, MUON>), (ns_finish<64, MUON>), g_big, dst, h, hd);
         }
     }
     return segmi_launch_status();
