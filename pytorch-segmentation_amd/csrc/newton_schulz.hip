@@ -22,13 +22,14 @@
 //
 // Symmetric products compute the tiles on and below the diagonal and store each twice.
 //
-// Layout.  A matrix row is a run of 128-byte lines; a line holds 32 consecutive values as 32 fp16 hi followed by 32 fp16 lo: one
-// line is one K step of a row, one DMA row of LDS, and one full HBM line.  Both dimensions are padded to 64 with zeros, so no
-// kernel but the first and the last knows a border.
+// Layout.  A line is 16 consecutive values of a row as 16 fp16 hi followed by 16 fp16 lo, 64 bytes: one matrix instruction's K, one
+// DMA row of LDS.  64 rows form a panel, in which line q of all 64 rows is one 4 KiB run, so that what a workgroup requests per step is
+// contiguous.  Both dimensions are padded to 64 with zeros: no kernel but the first and the last knows a border.
 #include "segmi_common.h"
 #include "lds_dma.h"
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 namespace {
 
@@ -37,7 +38,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int BATCH = 48;            // matrices per launch: their descriptors travel as kernel arguments (< 4 KiB)
 constexpr int MAX_GROUPS = 8;
-constexpr unsigned LINE = 128;
+constexpr unsigned LINE = 64, LINE_K = 16;   // bytes, values
 
 enum Buf { X = 0, T0, T1, A, Q, W, P0, P1 };
 
@@ -72,6 +73,10 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
     hi = (_Float16)v;
     lo = (_Float16)(v - (float)hi);
 }
+// where value k of a row lies
+__device__ __forceinline__ size_t at_line(unsigned lines, unsigned row, unsigned k) {
+    return ((size_t)((row >> 6) * lines + k / LINE_K) * 64 + (row & 63)) * LINE + k % LINE_K * 2;
+}
 // values k .. k+3 (k % 4 == 0) of a row
 __device__ __forceinline__ void store4(char* buf, unsigned lines, unsigned row, unsigned k, const float* v) {
     f16x4 hi, lo;
@@ -82,20 +87,20 @@ __device__ __forceinline__ void store4(char* buf, unsigned lines, unsigned row, 
         hi[x] = h;
         lo[x] = l;
     }
-    char* p = buf + ((size_t)row * lines + (k >> 5)) * LINE + (k & 31) * 2;
+    char* p = buf + at_line(lines, row, k);
     *reinterpret_cast<f16x4*>(p) = hi;
-    *reinterpret_cast<f16x4*>(p + 64) = lo;
+    *reinterpret_cast<f16x4*>(p + LINE / 2) = lo;
 }
 __device__ __forceinline__ void store1(char* buf, unsigned lines, unsigned row, unsigned k, float v) {
     _Float16 h, l;
     split(v, h, l);
-    char* p = buf + ((size_t)row * lines + (k >> 5)) * LINE + (k & 31) * 2;
+    char* p = buf + at_line(lines, row, k);
     *reinterpret_cast<_Float16*>(p) = h;
-    *reinterpret_cast<_Float16*>(p + 64) = l;
+    *reinterpret_cast<_Float16*>(p + LINE / 2) = l;
 }
 __device__ __forceinline__ void load4(const char* buf, unsigned lines, unsigned row, unsigned k, float* v) {
-    const char* p = buf + ((size_t)row * lines + (k >> 5)) * LINE + (k & 31) * 2;
-    const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + 64);
+    const char* p = buf + at_line(lines, row, k);
+    const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + LINE / 2);
 #pragma unroll
     for (int x = 0; x < 4; ++x) v[x] = (float)hi[x] + (float)lo[x];
 }
@@ -226,7 +231,7 @@ __global__ __launch_bounds__(256) void ns_normalise(SourceBatch b, Hyper h, cons
     char* const base = b.ws + (size_t)s.base * 256;
     char* const direct = base + buffer_offset(s.inner_is_n ? X : T0, m, n);
     char* const turned = base + buffer_offset(s.inner_is_n ? T0 : X, m, n);
-    const unsigned lines_inner = pad64(s.inner) / 32, lines_outer = pad64(s.outer) / 32;
+    const unsigned lines_inner = pad64(s.inner) / LINE_K, lines_outer = pad64(s.outer) / LINE_K;
     const float mu = MUON ? (hd ? hd->mom[s.group] : h.mom[s.group]) : 0.f;
     const bool nest = MUON && b.nesterov;
     const bool vec = s.dtype == 0 && s.si == 1 && (s.so & 3) == 0 && (s.inner & 3) == 0 && ((size_t)s.src & 15) == 0 && ((size_t)s.mom & 15) == 0;
@@ -276,32 +281,57 @@ __global__ __launch_bounds__(256) void ns_normalise(SourceBatch b, Hyper h, cons
 }
 
 // ------------------------------------------------------------------------------------------------ products
-// One workgroup's BT x BT tile of L R^T over the lines q0 .. q1-1 of both operands: 4 waves in 2 x 2, two LDS stages of one line per
-// row.  LDS chunk c (16 B) of row r sits at c ^ ((r >> 1) & 7): 16 consecutive rows, which one ds_read_b128 phase reads, then
-// cover all 64 banks; the permutation is applied to the DMA's source address.
+// One workgroup's BT x BT tile of L R^T over the lines q0 .. q1-1 of both operands: 4 waves in 2 x 2, two workgroups per CU.  A step is
+// U lines, 16 KiB of LDS, four of which are in use: one is multiplied while the copies of the next three are on their way.
+// LDS chunk c (16 B) of a row sits at c ^ ((row >> 2) & 3): 16 consecutive rows, which one ds_read_b128 phase reads, then cover all 64 banks;
+// the permutation is applied to the copy's source address.
+// Per step: the wave waits for ITS copies of the step (those of two later ones may be in flight), the barrier makes all waves' visible
+// and the step before it free, and the copies of the step three ahead go there, one every few products: requested in one go the copies of
+// the waves keep each of them from issuing products for the 16 cycles a copy occupies the CU's address path.
 template <int BT>
 struct Tile {
     static constexpr int S = BT / 64;                    // 32 x 32 subtiles per wave and dimension
-    static constexpr unsigned STAGE = 2 * BT * LINE;
+    static constexpr int U = BT == 128 ? 1 : 2;          // lines per step
+    static constexpr unsigned ROWS = BT * LINE;          // bytes of an operand's line
+    static constexpr unsigned STAGE = 2 * ROWS * U, STAGES = 4;
+    static constexpr int PIECES = BT / 64;               // 1 KiB copies (16 rows) per wave, operand and line
+    static constexpr int PER = 2 * PIECES * U;           // copies per wave and step
+    static constexpr int PITCH = BT + 8;                 // see `park`
+    static constexpr unsigned SMEM = STAGES * STAGE > BT * PITCH * 4 ? STAGES * STAGE : BT * PITCH * 4;
     f32x16 acc[S][S];
+
+    // This wave's LDS reads are back and at most N of its copies are in flight; then every wave's are.  The builtin, not asm: the
+    // compiler counts the LDS reads with it and puts no second wait before their uses.
+    template <int N>
+    __device__ __forceinline__ static void wait_all() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
 
     // The two mixed products have an accumulator of their own, added at the end: the large sum is rounded a third as often.
     __device__ __forceinline__ void run(char* smem, const char* L, unsigned rows_l, const char* R, unsigned rows_r, unsigned lines,
                                         unsigned l0, unsigned r0, unsigned q0, unsigned q1) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int wr = wave >> 1, wc = wave & 1;
-        const unsigned pitch = lines * LINE;
-        const i32x4 rl = make_rsrc(L, rows_l * pitch), rr = make_rsrc(R, rows_r * pitch);
-        constexpr int PIECES = BT / 32;                  // 1 KiB pieces (8 rows) per wave and operand
+        const i32x4 rsl = make_rsrc(L, rows_l * lines * LINE), rsr = make_rsrc(R, rows_r * lines * LINE);
         unsigned off_l[PIECES], off_r[PIECES];
         const unsigned lds = lds_addr(smem);
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const unsigned row = (wave * PIECES + p) * 8 + (lane >> 3);
-            const unsigned chunk = (lane & 7) ^ ((row >> 1) & 7);
-            off_l[p] = (l0 + row) * pitch + chunk * 16;
-            off_r[p] = (r0 + row) * pitch + chunk * 16;
+            const unsigned row = (wave * PIECES + p) * 16 + (lane >> 2);
+            const unsigned chunk = (lane & 3) ^ ((row >> 2) & 3);
+            off_l[p] = (unsigned)at_line(lines, l0 + row, 0) + chunk * 16;      // beyond the last panel: beyond the range, zeros
+            off_r[p] = (unsigned)at_line(lines, r0 + row, 0) + chunk * 16;
         }
+        // copy c of step k into `stage`
+        auto copy = [&](unsigned k, unsigned stage, int c) {
+            const int u = c / (2 * PIECES), o = c / PIECES % 2, p = c % PIECES;
+            const unsigned at = lds + stage * STAGE + (2 * u + o) * ROWS + (wave * PIECES + p) * 1024, q = (q0 + k * U + u) * (64 * LINE);
+            if (o == 0) dma16s(rsl, off_l[p], q, at);
+            else dma16s(rsr, off_r[p], q, at);
+        };
         f32x16 mix[S][S];
 #pragma unroll
         for (int i = 0; i < S; ++i)
@@ -309,52 +339,61 @@ struct Tile {
             for (int j = 0; j < S; ++j)
 #pragma unroll
                 for (int x = 0; x < 16; ++x) acc[i][j][x] = mix[i][j][x] = 0.f;
-
-        auto issue = [&](unsigned q, unsigned stage) {
+        const unsigned n = (q1 - q0) / U;                // >= 2
 #pragma unroll
-            for (int p = 0; p < PIECES; ++p) {
-                const unsigned at = lds + stage * STAGE + (wave * PIECES + p) * 1024;
-                dma16s(rl, off_l[p], q * LINE, at);
-                dma16s(rr, off_r[p], q * LINE, at + BT * LINE);
-            }
-        };
-        __syncthreads();                                 // the caller may have used this LDS
-        issue(q0, 0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+        for (unsigned k = 0; k < STAGES - 1; ++k)
+            if (k < n)
+#pragma unroll
+                for (int c = 0; c < PER; ++c) copy(k, k, c);
         const int fr = lane & 31, fk = lane >> 5;
-        const int sw = (fr >> 1) & 7;                    // row bases are multiples of 32: the swizzle depends on the lane alone
-        for (unsigned q = q0; q < q1; ++q) {
-            const unsigned stage = (q - q0) & 1;
-            if (q + 1 < q1) issue(q + 1, stage ^ 1);
-            const char* const sl = smem + stage * STAGE + (wr * S * 32 + fr) * LINE;
-            const char* const sr = smem + stage * STAGE + BT * LINE + (wc * S * 32 + fr) * LINE;
+        const int sw = (fr >> 2) & 3;                    // row bases are multiples of 32: the permutation depends on the lane alone
+        const int hi = (fk ^ sw) * 16, lo = ((fk + 2) ^ sw) * 16;
+        const char* const sl = smem + (wr * S * 32 + fr) * LINE;
+        const char* const sr = smem + ROWS + (wc * S * 32 + fr) * LINE;
+        auto step = [&](unsigned k, auto more) {
+            const unsigned at = (k % STAGES) * STAGE;
+            f16x8 lh[U][S], ll[U][S], rh[U][S], rl[U][S];
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                const int hi = ((ks * 2 + fk) ^ sw) * 16, lo = ((ks * 2 + fk + 4) ^ sw) * 16;
-                f16x8 lh[S], ll[S], rh[S], rl8[S];
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int i = 0; i < S; ++i) {
-                    lh[i] = *reinterpret_cast<const f16x8*>(sl + i * 32 * LINE + hi);
-                    ll[i] = *reinterpret_cast<const f16x8*>(sl + i * 32 * LINE + lo);
-                    rh[i] = *reinterpret_cast<const f16x8*>(sr + i * 32 * LINE + hi);
-                    rl8[i] = *reinterpret_cast<const f16x8*>(sr + i * 32 * LINE + lo);
+                    const unsigned o = at + 2 * u * ROWS + i * 32 * LINE;
+                    lh[u][i] = *reinterpret_cast<const f16x8*>(sl + o + hi);
+                    rh[u][i] = *reinterpret_cast<const f16x8*>(sr + o + hi);
+                    ll[u][i] = *reinterpret_cast<const f16x8*>(sl + o + lo);
+                    rl[u][i] = *reinterpret_cast<const f16x8*>(sr + o + lo);
                 }
+            __builtin_amdgcn_sched_barrier(0);
+            constexpr int EACH = 3 * S * S * U / PER;
+            int done = 0;
 #pragma unroll
-                for (int i = 0; i < S; ++i)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int j = 0; j < S; ++j) mix[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll[i], rh[j], mix[i][j], 0, 0, 0);
+                for (int t = 0; t < 3; ++t)
 #pragma unroll
-                for (int i = 0; i < S; ++i)
+                    for (int i = 0; i < S; ++i)
 #pragma unroll
-                    for (int j = 0; j < S; ++j) mix[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[i], rl8[j], mix[i][j], 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < S; ++i)
-#pragma unroll
-                    for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[i], rh[j], acc[i][j], 0, 0, 0);
-            }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
+                        for (int j = 0; j < S; ++j) {
+                            if (t == 0) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[u][i], rh[u][j], acc[i][j], 0, 0, 0);
+                            if (t == 1) mix[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll[u][i], rh[u][j], mix[i][j], 0, 0, 0);
+                            if (t == 2) mix[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[u][i], rl[u][j], mix[i][j], 0, 0, 0);
+                            if (decltype(more)::value && (((u * 3 + t) * S + i) * S + j) % EACH == 0 && done < PER) {
+                                __builtin_amdgcn_sched_barrier(0);
+                                copy(k + STAGES - 1, (k + STAGES - 1) % STAGES, done++);
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                        }
+        };
+        unsigned k = 0;
+        for (; k + STAGES - 1 < n; ++k) {
+            wait_all<2 * PER>();
+            step(k, std::true_type{});
+        }
+        for (; k < n; ++k) {                             // everything is under way or here
+            if (k + 2 < n) wait_all<2 * PER>();
+            else if (k + 1 < n) wait_all<PER>();
+            else wait_all<0>();
+            step(k, std::false_type{});
         }
 #pragma unroll
         for (int i = 0; i < S; ++i)
@@ -364,20 +403,42 @@ struct Tile {
                 for (int x = 0; x < 16; ++x) acc[i][j][x] += mix[i][j][x];
     }
 
-    // f(i, j, g, row, col): values acc[i][j][4 g .. 4 g + 3] are rows row .. row+3 of column col (tile-relative)
+    // f(row, col, v) per 32 x 32 subtile: v[4 g + x] is row `row` + 8 g + x of column `col` (tile-relative)
     template <typename F>
-    __device__ __forceinline__ void each4(F f) const {
+    __device__ __forceinline__ void each(F f) const {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 #pragma unroll
         for (int i = 0; i < S; ++i)
 #pragma unroll
-            for (int j = 0; j < S; ++j)
+            for (int j = 0; j < S; ++j) {
+                float v[16];
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int row = ((wave >> 1) * S + i) * 32 + 8 * g + 4 * (lane >> 5), col = ((wave & 1) * S + j) * 32 + (lane & 31);
-                    const float v[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                    f(row, col, v);
-                }
+                for (int x = 0; x < 16; ++x) v[x] = acc[i][j][x];
+                f(((wave >> 1) * S + i) * 32 + 4 * (lane >> 5), ((wave & 1) * S + j) * 32 + (lane & 31), v);
+            }
+    }
+
+    // Turning a tile round in LDS: a lane holds runs of rows of one column, a row's line wants runs of columns.  `park` keeps the pair
+    // of a value, `store_rows` writes all parked rows, 16 B a lane.  Pitch: 4 rows apart is 32 banks apart.
+    __device__ __forceinline__ static void park(char* smem, int row, int col, float v) {
+        _Float16 h, l;
+        split(v, h, l);
+        reinterpret_cast<unsigned*>(smem)[row * PITCH + col] = __builtin_bit_cast(unsigned short, h) | (unsigned)__builtin_bit_cast(unsigned short, l) << 16;
+    }
+    __device__ __forceinline__ static void store_rows(const char* smem, char* out, unsigned lines, unsigned r0, unsigned c0, unsigned rows, unsigned cols) {
+        __syncthreads();
+        constexpr int PER_ROW = BT / 8;
+        const int c = (threadIdx.x % PER_ROW) * 8;
+        for (int r = threadIdx.x / PER_ROW; r < BT; r += 256 / PER_ROW) {
+            if (r0 + r >= rows || c0 + c >= cols) continue;
+            const uint4 p = *reinterpret_cast<const uint4*>(smem + (r * PITCH + c) * 4), q = *reinterpret_cast<const uint4*>(smem + (r * PITCH + c) * 4 + 16);
+            uint4 hi, lo;
+            hi.x = (p.x & 0xFFFFu) | p.y << 16; hi.y = (p.z & 0xFFFFu) | p.w << 16; hi.z = (q.x & 0xFFFFu) | q.y << 16; hi.w = (q.z & 0xFFFFu) | q.w << 16;
+            lo.x = p.x >> 16 | (p.y & 0xFFFF0000u); lo.y = p.z >> 16 | (p.w & 0xFFFF0000u); lo.z = q.x >> 16 | (q.y & 0xFFFF0000u); lo.w = q.z >> 16 | (q.w & 0xFFFF0000u);
+            char* const at = out + at_line(lines, r0 + r, c0 + c);
+            *reinterpret_cast<uint4*>(at) = hi;
+            *reinterpret_cast<uint4*>(at + LINE / 2) = lo;
+        }
     }
 };
 
@@ -407,31 +468,37 @@ struct Product {
 // m x m products (all operands symmetric): A^2 with the polynomial's epilogue, Q A, W Q, P Q.
 template <int BT, bool POLY>
 __global__ __launch_bounds__(256, 2) void ns_square_product(Batch b, Product pr) {
-    __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<BT>::STAGE];
+    __shared__ __attribute__((aligned(1024))) char smem[Tile<BT>::SMEM];
     const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
     const Item s = b.item[find_item(b, wg)];
     char* const base = b.ws + (size_t)s.base * 256;
-    const unsigned M = pad64(s.m), lines = M / 32;
+    const unsigned M = pad64(s.m), lines = M / LINE_K;
     unsigned ti, tj;
     lower_tile(wg - s.first, ti, tj);
     Tile<BT> t;
     t.run(smem, base + buffer_offset(pr.l, s.m, s.n), M, base + buffer_offset(pr.r, s.m, s.n), M, lines, ti * BT, tj * BT, 0, lines);
     char* const out = base + buffer_offset(pr.out, s.m, s.n);
     const char* const a = base + buffer_offset(A, s.m, s.n);
-    t.each4([&](int row, int col, const float* acc) {
+    const bool mirror = ti != tj;
+    if (mirror) __syncthreads();                         // every wave is done with the stages
+    t.each([&](int row, int col, float* v) {
         const unsigned r = ti * BT + row, c = tj * BT + col;
-        if (r >= M || c >= M) return;
-        float v[4];
+        const bool in = r < M && c < M;                  // (all 32 rows of a subtile or none)
+        float av[16];
+        if (POLY && in)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = acc[x] * pr.scale;
-        if (POLY) {
-            float av[4];
-            load4(a, lines, c, r, av);
+            for (int g = 0; g < 4; ++g) load4(a, lines, c, r + 8 * g, av + 4 * g);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) v[x] += pr.lin * av[x] + (r + x == c && c < (unsigned)s.m ? pr.ident : 0.f);
+        for (int x = 0; x < 16; ++x) {
+            v[x] *= pr.scale;
+            if (POLY) v[x] += pr.lin * av[x] + (r + 8 * (x >> 2) + (x & 3) == c && c < (unsigned)s.m ? pr.ident : 0.f);
+            if (mirror) Tile<BT>::park(smem, row + 8 * (x >> 2) + (x & 3), col, v[x]);
         }
-        store_symmetric(out, lines, r, c, v, ti != tj);
+        if (in)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) store4(out, lines, c, r + 8 * g, v + 4 * g);
     });
+    if (mirror) Tile<BT>::store_rows(smem, out, lines, ti * BT, tj * BT, M, M);
 }
 
 // Gram products A = X X^T: few tiles, long sums.  The sum is cut into `splits` runs of lines, each workgroup leaves its fp32 tile in
@@ -451,11 +518,11 @@ struct GramBatch {
 
 template <int BT>
 __global__ __launch_bounds__(256, 2) void ns_gram(GramBatch b) {
-    __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<BT>::STAGE];
+    __shared__ __attribute__((aligned(1024))) char smem[Tile<BT>::SMEM];
     const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
     const GramItem s = b.item[find_item(b, wg)];
     const char* const x = b.ws + (size_t)s.base * 256;
-    const unsigned M = pad64(s.m), lines = pad64(s.n) / 32;
+    const unsigned M = pad64(s.m), lines = pad64(s.n) / LINE_K;
     const unsigned u = wg - s.first, k = u / s.tiles, tile = u - k * s.tiles;      // the tiles of one run are neighbours: they share its lines
     unsigned ti, tj;
     lower_tile(tile, ti, tj);
@@ -509,40 +576,52 @@ __global__ __launch_bounds__(256) void ns_gram_reduce(GramBatch b) {
     const unsigned M = pad64(s.m);
     const unsigned row = ti * BT + (sub / (BT / 32)) * 32 + 8 * g + 4 * (lane >> 5), col = tj * BT + (sub % (BT / 32)) * 32 + (lane & 31);
     if (row >= M || col >= M) return;
-    store_symmetric(b.ws + (size_t)s.base * 256 + buffer_offset(A, s.m, s.n), M / 32, row, col, r4, ti != tj);
+    store_symmetric(b.ws + (size_t)s.base * 256 + buffer_offset(A, s.m, s.n), M / LINE_K, row, col, r4, ti != tj);
+}
+
+// The tiles of a product with P in strips of 8 rows of tiles, column by column: what an XCD works on at a time (32 tiles of 128) is then
+// nearly square, and its L2 serves every panel to several workgroups (4096 x 4096: 409 -> 257 us for the copies alone).
+__device__ __forceinline__ void big_tile(unsigned u, unsigned down, unsigned across, unsigned& ti, unsigned& tj) {
+    const unsigned g = u / (8 * across), left = down - 8 * g, h = left < 8 ? left : 8, v = u - 8 * g * across;
+    tj = v / h;
+    ti = 8 * g + v - tj * h;
 }
 
 // X <- alpha X + P X between segments (alpha = 0 where P holds the identity's part): both orders again (T1 from T0, X in place:
 // no workgroup reads X)
 template <int BT>
 __global__ __launch_bounds__(256, 2) void ns_apply(Batch b, int p, int tin, int tout, float scale, float alpha) {
-    __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<BT>::STAGE];
+    __shared__ __attribute__((aligned(1024))) char smem[Tile<BT>::SMEM];
     const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
     const Item s = b.item[find_item(b, wg)];
     char* const base = b.ws + (size_t)s.base * 256;
     const unsigned M = pad64(s.m), N = pad64(s.n);
-    const unsigned down = (M + BT - 1) / BT, u = wg - s.first, tj = u / down, ti = u - tj * down;
+    unsigned ti, tj;
+    big_tile(wg - s.first, (M + BT - 1) / BT, (N + BT - 1) / BT, ti, tj);
     Tile<BT> t;
-    t.run(smem, base + buffer_offset(p, s.m, s.n), M, base + buffer_offset(tin, s.m, s.n), N, M / 32, ti * BT, tj * BT, 0, M / 32);
+    t.run(smem, base + buffer_offset(p, s.m, s.n), M, base + buffer_offset(tin, s.m, s.n), N, M / LINE_K, ti * BT, tj * BT, 0, M / LINE_K);
     char* const xo = base;
     char* const to = base + buffer_offset(tout, s.m, s.n);
     const char* const ti4 = base + buffer_offset(tin, s.m, s.n);
-    t.each4([&](int row, int col, const float* acc) {
+    __syncthreads();
+    t.each([&](int row, int col, float* v) {
         const unsigned r = ti * BT + row, c = tj * BT + col;
-        if (r >= M || c >= N) return;
-        float v[4];
+        const bool in = r < M && c < N;
+        float old[16];
+        if (alpha != 0.f && in)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = acc[x] * scale;
-        if (alpha != 0.f) {
-            float old[4];
-            load4(ti4, M / 32, c, r, old);
+            for (int g = 0; g < 4; ++g) load4(ti4, M / LINE_K, c, r + 8 * g, old + 4 * g);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) v[x] = fmaf(alpha, old[x], v[x]);
+        for (int x = 0; x < 16; ++x) {
+            v[x] *= scale;
+            if (alpha != 0.f && in) v[x] = fmaf(alpha, old[x], v[x]);
+            Tile<BT>::park(smem, row + 8 * (x >> 2) + (x & 3), col, v[x]);
         }
-        store4(to, M / 32, c, r, v);
+        if (in)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) store1(xo, N / 32, r + x, c, v[x]);
+            for (int g = 0; g < 4; ++g) store4(to, M / LINE_K, c, r + 8 * g, v + 4 * g);
     });
+    Tile<BT>::store_rows(smem, xo, N / LINE_K, ti * BT, tj * BT, M, N);
 }
 
 // the last product goes straight to where the caller wants it
@@ -566,17 +645,18 @@ struct TargetBatch {
 // MUON: param = param (1 - lr wd) - lr factor O, else dst = O
 template <int BT, bool MUON>
 __global__ __launch_bounds__(256, 2) void ns_finish(TargetBatch b, Hyper h, const Hyper* __restrict__ hd) {
-    __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<BT>::STAGE];
+    __shared__ __attribute__((aligned(1024))) char smem[Tile<BT>::SMEM];
     const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
     const Target s = b.item[find_item(b, wg)];
     const char* const base = b.ws + (size_t)s.base * 256;
     const unsigned M = pad64(s.m), N = pad64(s.n);
-    const unsigned down = (M + BT - 1) / BT, u = wg - s.first, tj = u / down, ti = u - tj * down;
+    unsigned ti, tj;
+    big_tile(wg - s.first, (M + BT - 1) / BT, (N + BT - 1) / BT, ti, tj);
     const char* const P = base + buffer_offset(b.p, s.m, s.n);
     const char* const T = base + buffer_offset(b.tin, s.m, s.n);
     Tile<BT> t;
-    if (s.turned) t.run(smem, T, N, P, M, M / 32, tj * BT, ti * BT, 0, M / 32);
-    else t.run(smem, P, M, T, N, M / 32, ti * BT, tj * BT, 0, M / 32);
+    if (s.turned) t.run(smem, T, N, P, M, M / LINE_K, tj * BT, ti * BT, 0, M / LINE_K);
+    else t.run(smem, P, M, T, N, M / LINE_K, ti * BT, tj * BT, 0, M / LINE_K);
     const unsigned r0 = (s.turned ? tj : ti) * BT, c0 = (s.turned ? ti : tj) * BT;
     const unsigned rows = s.turned ? s.n : s.m, cols = s.turned ? s.m : s.n;
     const long sr = s.turned ? s.sj : s.si, sc = s.turned ? s.si : s.sj;
@@ -587,26 +667,30 @@ __global__ __launch_bounds__(256, 2) void ns_finish(TargetBatch b, Hyper h, cons
         step = lr * s.factor;
     }
     const char* const old = s.turned ? base : T;         // row c of it, values r .. r+3: X's own order, or the other one
-    const unsigned old_lines = (s.turned ? N : M) / 32;
-    t.each4([&](int row, int col, const float* acc) {
-        const unsigned c = c0 + col;
-        if (c >= cols || r0 + row >= rows) return;
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
-        if (b.alpha != 0.f) load4(old, old_lines, c, r0 + row, o);
+    const unsigned old_lines = (s.turned ? N : M) / LINE_K;
+    t.each([&](int row, int col, float* v) {
+        const unsigned c = c0 + col, r = r0 + row;
+        if (c >= cols || r >= rows) return;              // (r is the lane's first row)
+        float old4[16], before[16];
+        if (b.alpha != 0.f)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const unsigned r = r0 + row + x;
-            if (r >= rows) break;
-            const float v = fmaf(b.alpha, o[x], acc[x] * b.scale);
-            const long at = (long)r * sr + (long)c * sc;
-            if (MUON) {
-                float* const p = static_cast<float*>(s.dst) + at;
-                *p = fmaf(-step, v, *p * keep);
-            } else if (s.dtype) {
-                static_cast<unsigned short*>(s.dst)[at] = f32_to_bf16(v);
-            } else {
-                static_cast<float*>(s.dst)[at] = v;
+            for (int g = 0; g < 4; ++g) load4(old, old_lines, c, r + 8 * g, old4 + 4 * g);    // padded rows: in the buffer
+        if (MUON)                                        // all loads first: behind a store they would wait for it
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const unsigned rr = r + 8 * (x >> 2) + (x & 3);
+                if (rr < rows) before[x] = static_cast<const float*>(s.dst)[(long)rr * sr + (long)c * sc];
             }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const unsigned rr = r + 8 * (x >> 2) + (x & 3);
+            if (rr >= rows) continue;
+            float o = v[x] * b.scale;
+            if (b.alpha != 0.f) o = fmaf(b.alpha, old4[x], o);
+            const long at = (long)rr * sr + (long)c * sc;
+            if (MUON) static_cast<float*>(s.dst)[at] = fmaf(-step, o, before[x] * keep);
+            else if (s.dtype) static_cast<unsigned short*>(s.dst)[at] = f32_to_bf16(o);
+            else static_cast<float*>(s.dst)[at] = o;
         }
     });
 }
@@ -710,7 +794,7 @@ int tile_size(const Shape* s, int count, F tiles) {
         else hipLaunchKernelGGL(kernel64, dim3(grid), dim3(256), 0, st, __VA_ARGS__);                          \
     } while (0)
 
-// runs of a Gram product: enough workgroups to fill the chip, no run shorter than 8 lines
+// runs of a Gram product: enough workgroups to fill the chip, no run shorter than 16 lines
 struct GramPlan {
     int bt;
     unsigned run;
@@ -719,12 +803,12 @@ GramPlan gram_plan(const Shape* s, int count) {
     GramPlan best{64, 0};
     double work128 = 0.0, work64 = 0.0;
     for (int i = 0; i < count; ++i) {
-        work128 += (double)low_tiles(s[i].m, 128) * (pad64(s[i].n) / 32);
-        work64 += (double)low_tiles(s[i].m, 64) * (pad64(s[i].n) / 32);
+        work128 += (double)low_tiles(s[i].m, 128) * (pad64(s[i].n) / LINE_K);
+        work64 += (double)low_tiles(s[i].m, 64) * (pad64(s[i].n) / LINE_K);
     }
-    best.bt = work128 / 8.0 >= 512.0 ? 128 : 64;
-    const double run = std::ceil((best.bt == 128 ? work128 / 1024.0 : work64 / 2048.0));
-    best.run = run < 8.0 ? 8u : (unsigned)run;
+    best.bt = work128 / 16.0 >= 512.0 ? 128 : 64;
+    const double run = std::ceil((best.bt == 128 ? work128 / 1024.0 : work64 / 2048.0) / 4.0) * 4.0;
+    best.run = run < 16.0 ? 16u : (unsigned)run;         // whole steps of a tile
     return best;
 }
 
@@ -735,7 +819,7 @@ Plan plan_batch(const Shape* s, int count) {
     size_t parts = 0, slots = 0, mats = 0;
     const GramPlan g = gram_plan(s, count);
     for (int i = 0; i < count; ++i) {
-        const unsigned lines = pad64(s[i].n) / 32;
+        const unsigned lines = pad64(s[i].n) / LINE_K;
         parts += (size_t)segmi_cdiv(s[i].outer, 64) * segmi_cdiv(s[i].inner, 256);
         slots += (size_t)low_tiles(s[i].m, g.bt) * segmi_cdiv(lines, g.run);
         mats += 3 * big_bytes(s[i].m, s[i].n) + 5 * square_bytes(s[i].m);
@@ -766,7 +850,7 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
     size_t base = 0;
     for (int i = 0; i < count; ++i) {
         const Shape& s = shapes[i];
-        const unsigned lines = pad64(s.n) / 32, low = low_tiles(s.m, gp.bt), splits = segmi_cdiv(lines, gp.run);
+        const unsigned lines = pad64(s.n) / LINE_K, low = low_tiles(s.m, gp.bt), splits = segmi_cdiv(lines, gp.run);
         const unsigned b256 = (unsigned)(base / 256);
         const unsigned units = segmi_cdiv(s.outer, 64) * segmi_cdiv(s.inner, 256);
         src.item[i].base = dst.item[i].base = b256;
