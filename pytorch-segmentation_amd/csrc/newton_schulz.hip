@@ -27,9 +27,10 @@
 // contiguous.  Both dimensions are padded to 64 with zeros: no kernel but the first and the last knows a border.
 #include "segmi_common.h"
 #include "lds_dma.h"
+#include <algorithm>
 #include <cmath>
-#include <cstring>
 #include <type_traits>
+#include <vector>
 
 namespace {
 
@@ -61,7 +62,8 @@ __host__ __device__ inline size_t buffer_offset(int buf, int m, int n) {
     return buf < A ? (size_t)buf * big_bytes(m, n) : 3 * big_bytes(m, n) + (size_t)(buf - A) * square_bytes(m);
 }
 
-// lane l looks at item l: one load and one ballot instead of a search
+// lane l looks at item l: one load and one ballot instead of a search.  (Workgroups are dealt to the XCDs within each matrix, by
+// xcd_swizzle of the number inside it: an XCD gets a run of neighbouring tiles of EVERY matrix, however unequal their sums are.)
 template <typename B>
 __device__ __forceinline__ int find_item(const B& b, unsigned wg) {
     const int lane = threadIdx.x & 63;
@@ -288,12 +290,16 @@ __global__ __launch_bounds__(256) void ns_normalise(SourceBatch b, Hyper h, cons
 // Per step: the wave waits for ITS copies of the step (those of two later ones may be in flight), the barrier makes all waves' visible
 // and the step before it free, and the copies of the step three ahead go there, one every few products: requested in one go the copies of
 // the waves keep each of them from issuing products for the 16 cycles a copy occupies the CU's address path.
-template <int BT>
+struct Wide { static constexpr int BT = 128, U = 1, PER_CU = 2; static constexpr unsigned STAGES = 4; };
+struct Many { static constexpr int BT = 64, U = 1, PER_CU = 4; static constexpr unsigned STAGES = 4; };
+struct Few { static constexpr int BT = 64, U = 2, PER_CU = 1; static constexpr unsigned STAGES = 8; };
+
+template <typename C>
 struct Tile {
+    static constexpr int BT = C::BT, U = C::U;           // U: lines per step
     static constexpr int S = BT / 64;                    // 32 x 32 subtiles per wave and dimension
-    static constexpr int U = BT == 128 ? 1 : 2;          // lines per step
     static constexpr unsigned ROWS = BT * LINE;          // bytes of an operand's line
-    static constexpr unsigned STAGE = 2 * ROWS * U, STAGES = 4;
+    static constexpr unsigned STAGE = 2 * ROWS * U, STAGES = C::STAGES;
     static constexpr int PIECES = BT / 64;               // 1 KiB copies (16 rows) per wave, operand and line
     static constexpr int PER = 2 * PIECES * U;           // copies per wave and step
     static constexpr int PITCH = BT + 8;                 // see `park`
@@ -386,13 +392,19 @@ struct Tile {
         };
         unsigned k = 0;
         for (; k + STAGES - 1 < n; ++k) {
-            wait_all<2 * PER>();
+            wait_all<(STAGES - 2) * PER>();
             step(k, std::true_type{});
         }
         for (; k < n; ++k) {                             // everything is under way or here
-            if (k + 2 < n) wait_all<2 * PER>();
-            else if (k + 1 < n) wait_all<PER>();
-            else wait_all<0>();
+            switch (n - 1 - k < STAGES - 2 ? n - 1 - k : STAGES - 2) {
+                case 0: wait_all<0>(); break;
+                case 1: wait_all<PER>(); break;
+                case 2: wait_all<2 * PER>(); break;
+                case 3: wait_all<3 * PER>(); break;
+                case 4: wait_all<4 * PER>(); break;
+                case 5: wait_all<5 * PER>(); break;
+                default: wait_all<6 * PER>(); break;
+            }
             step(k, std::false_type{});
         }
 #pragma unroll
@@ -466,16 +478,16 @@ struct Product {
 };
 
 // m x m products (all operands symmetric): A^2 with the polynomial's epilogue, Q A, W Q, P Q.
-template <int BT, bool POLY>
-__global__ __launch_bounds__(256, 2) void ns_square_product(Batch b, Product pr) {
-    __shared__ __attribute__((aligned(1024))) char smem[Tile<BT>::SMEM];
-    const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
-    const Item s = b.item[find_item(b, wg)];
+template <typename C, bool POLY>
+__global__ __launch_bounds__(256, C::PER_CU) void ns_square_product(Batch b, Product pr) {
+    constexpr int BT = C::BT;
+    __shared__ __attribute__((aligned(1024))) char smem[Tile<C>::SMEM];
+    const Item s = b.item[find_item(b, blockIdx.x)];
     char* const base = b.ws + (size_t)s.base * 256;
-    const unsigned M = pad64(s.m), lines = M / LINE_K;
+    const unsigned M = pad64(s.m), lines = M / LINE_K, rows = (M + BT - 1) / BT;
     unsigned ti, tj;
-    lower_tile(wg - s.first, ti, tj);
-    Tile<BT> t;
+    lower_tile(xcd_swizzle(blockIdx.x - s.first, rows * (rows + 1) / 2), ti, tj);
+    Tile<C> t;
     t.run(smem, base + buffer_offset(pr.l, s.m, s.n), M, base + buffer_offset(pr.r, s.m, s.n), M, lines, ti * BT, tj * BT, 0, lines);
     char* const out = base + buffer_offset(pr.out, s.m, s.n);
     const char* const a = base + buffer_offset(A, s.m, s.n);
@@ -492,13 +504,13 @@ __global__ __launch_bounds__(256, 2) void ns_square_product(Batch b, Product pr)
         for (int x = 0; x < 16; ++x) {
             v[x] *= pr.scale;
             if (POLY) v[x] += pr.lin * av[x] + (r + 8 * (x >> 2) + (x & 3) == c && c < (unsigned)s.m ? pr.ident : 0.f);
-            if (mirror) Tile<BT>::park(smem, row + 8 * (x >> 2) + (x & 3), col, v[x]);
+            if (mirror) Tile<C>::park(smem, row + 8 * (x >> 2) + (x & 3), col, v[x]);
         }
         if (in)
 #pragma unroll
             for (int g = 0; g < 4; ++g) store4(out, lines, c, r + 8 * g, v + 4 * g);
     });
-    if (mirror) Tile<BT>::store_rows(smem, out, lines, ti * BT, tj * BT, M, M);
+    if (mirror) Tile<C>::store_rows(smem, out, lines, ti * BT, tj * BT, M, M);
 }
 
 // Gram products A = X X^T: few tiles, long sums.  The sum is cut into `splits` runs of lines, each workgroup leaves its fp32 tile in
@@ -516,21 +528,21 @@ struct GramBatch {
     GramItem item[BATCH];
 };
 
-template <int BT>
-__global__ __launch_bounds__(256, 2) void ns_gram(GramBatch b) {
-    __shared__ __attribute__((aligned(1024))) char smem[Tile<BT>::SMEM];
-    const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
-    const GramItem s = b.item[find_item(b, wg)];
+template <typename C>
+__global__ __launch_bounds__(256, C::PER_CU) void ns_gram(GramBatch b) {
+    constexpr int BT = C::BT;
+    __shared__ __attribute__((aligned(1024))) char smem[Tile<C>::SMEM];
+    const GramItem s = b.item[find_item(b, blockIdx.x)];
     const char* const x = b.ws + (size_t)s.base * 256;
     const unsigned M = pad64(s.m), lines = pad64(s.n) / LINE_K;
-    const unsigned u = wg - s.first, k = u / s.tiles, tile = u - k * s.tiles;      // the tiles of one run are neighbours: they share its lines
+    const unsigned u = xcd_swizzle(blockIdx.x - s.first, s.tiles * s.splits), k = u / s.tiles, tile = u - k * s.tiles;      // the tiles of one run are neighbours: they share its lines
     unsigned ti, tj;
     lower_tile(tile, ti, tj);
-    Tile<BT> t;
+    Tile<C> t;
     const unsigned q0 = k * s.run, q1 = q0 + s.run < lines ? q0 + s.run : lines;
     t.run(smem, x, M, x, M, lines, ti * BT, tj * BT, q0, q1);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    constexpr int S = Tile<BT>::S;
+    constexpr int S = Tile<C>::S;
     float* const out = b.partial + ((size_t)s.part + (size_t)tile * s.splits + k) * (BT * BT);
 #pragma unroll
     for (int i = 0; i < S; ++i)
@@ -582,6 +594,7 @@ __global__ __launch_bounds__(256) void ns_gram_reduce(GramBatch b) {
 // The tiles of a product with P in strips of 8 rows of tiles, column by column: what an XCD works on at a time (32 tiles of 128) is then
 // nearly square, and its L2 serves every panel to several workgroups (4096 x 4096: 409 -> 257 us for the copies alone).
 __device__ __forceinline__ void big_tile(unsigned u, unsigned down, unsigned across, unsigned& ti, unsigned& tj) {
+    u = xcd_swizzle(u, down * across);
     const unsigned g = u / (8 * across), left = down - 8 * g, h = left < 8 ? left : 8, v = u - 8 * g * across;
     tj = v / h;
     ti = 8 * g + v - tj * h;
@@ -589,16 +602,16 @@ __device__ __forceinline__ void big_tile(unsigned u, unsigned down, unsigned acr
 
 // X <- alpha X + P X between segments (alpha = 0 where P holds the identity's part): both orders again (T1 from T0, X in place:
 // no workgroup reads X)
-template <int BT>
-__global__ __launch_bounds__(256, 2) void ns_apply(Batch b, int p, int tin, int tout, float scale, float alpha) {
-    __shared__ __attribute__((aligned(1024))) char smem[Tile<BT>::SMEM];
-    const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
-    const Item s = b.item[find_item(b, wg)];
+template <typename C>
+__global__ __launch_bounds__(256, C::PER_CU) void ns_apply(Batch b, int p, int tin, int tout, float scale, float alpha) {
+    constexpr int BT = C::BT;
+    __shared__ __attribute__((aligned(1024))) char smem[Tile<C>::SMEM];
+    const Item s = b.item[find_item(b, blockIdx.x)];
     char* const base = b.ws + (size_t)s.base * 256;
     const unsigned M = pad64(s.m), N = pad64(s.n);
     unsigned ti, tj;
-    big_tile(wg - s.first, (M + BT - 1) / BT, (N + BT - 1) / BT, ti, tj);
-    Tile<BT> t;
+    big_tile(blockIdx.x - s.first, (M + BT - 1) / BT, (N + BT - 1) / BT, ti, tj);
+    Tile<C> t;
     t.run(smem, base + buffer_offset(p, s.m, s.n), M, base + buffer_offset(tin, s.m, s.n), N, M / LINE_K, ti * BT, tj * BT, 0, M / LINE_K);
     char* const xo = base;
     char* const to = base + buffer_offset(tout, s.m, s.n);
@@ -615,13 +628,13 @@ __global__ __launch_bounds__(256, 2) void ns_apply(Batch b, int p, int tin, int 
         for (int x = 0; x < 16; ++x) {
             v[x] *= scale;
             if (alpha != 0.f && in) v[x] = fmaf(alpha, old[x], v[x]);
-            Tile<BT>::park(smem, row + 8 * (x >> 2) + (x & 3), col, v[x]);
+            Tile<C>::park(smem, row + 8 * (x >> 2) + (x & 3), col, v[x]);
         }
         if (in)
 #pragma unroll
             for (int g = 0; g < 4; ++g) store4(to, M / LINE_K, c, r + 8 * g, v + 4 * g);
     });
-    Tile<BT>::store_rows(smem, xo, N / LINE_K, ti * BT, tj * BT, M, N);
+    Tile<C>::store_rows(smem, xo, N / LINE_K, ti * BT, tj * BT, M, N);
 }
 
 // the last product goes straight to where the caller wants it
@@ -643,18 +656,18 @@ struct TargetBatch {
 };
 
 // MUON: param = param (1 - lr wd) - lr factor O, else dst = O
-template <int BT, bool MUON>
-__global__ __launch_bounds__(256, 2) void ns_finish(TargetBatch b, Hyper h, const Hyper* __restrict__ hd) {
-    __shared__ __attribute__((aligned(1024))) char smem[Tile<BT>::SMEM];
-    const unsigned wg = xcd_swizzle(blockIdx.x, gridDim.x);
-    const Target s = b.item[find_item(b, wg)];
+template <typename C, bool MUON>
+__global__ __launch_bounds__(256, C::PER_CU) void ns_finish(TargetBatch b, Hyper h, const Hyper* __restrict__ hd) {
+    constexpr int BT = C::BT;
+    __shared__ __attribute__((aligned(1024))) char smem[Tile<C>::SMEM];
+    const Target s = b.item[find_item(b, blockIdx.x)];
     const char* const base = b.ws + (size_t)s.base * 256;
     const unsigned M = pad64(s.m), N = pad64(s.n);
     unsigned ti, tj;
-    big_tile(wg - s.first, (M + BT - 1) / BT, (N + BT - 1) / BT, ti, tj);
+    big_tile(blockIdx.x - s.first, (M + BT - 1) / BT, (N + BT - 1) / BT, ti, tj);
     const char* const P = base + buffer_offset(b.p, s.m, s.n);
     const char* const T = base + buffer_offset(b.tin, s.m, s.n);
-    Tile<BT> t;
+    Tile<C> t;
     if (s.turned) t.run(smem, T, N, P, M, M / LINE_K, tj * BT, ti * BT, 0, M / LINE_K);
     else t.run(smem, P, M, T, N, M / LINE_K, ti * BT, tj * BT, 0, M / LINE_K);
     const unsigned r0 = (s.turned ? tj : ti) * BT, c0 = (s.turned ? ti : tj) * BT;
@@ -781,35 +794,47 @@ unsigned tiles_of(int m, int bt) { return (pad64(m) + bt - 1) / bt; }
 unsigned low_tiles(int m, int bt) { const unsigned t = tiles_of(m, bt); return t * (t + 1) / 2; }
 unsigned big_tiles(const Shape& s, int bt) { return tiles_of(s.m, bt) * tiles_of(s.n, bt); }
 
-// Tile size of a launch: 128 x 128 where that still gives every CU a workgroup
+// Which tiles a launch runs on (see Tile)
+enum Config { WIDE, MANY, FEW };
+int tile_of(Config c) { return c == WIDE ? 128 : 64; }
 template <typename F>
-int tile_size(const Shape* s, int count, F tiles) {
-    size_t t = 0;
-    for (int i = 0; i < count; ++i) t += tiles(s[i], 128);
-    return t >= SEGMI_NUM_CU ? 128 : 64;
+Config config_of(const Shape* s, int count, F tiles) {
+    size_t wide = 0, many = 0;
+    for (int i = 0; i < count; ++i) {
+        wide += tiles(s[i], 128);
+        many += tiles(s[i], 64);
+    }
+    return wide >= SEGMI_NUM_CU ? WIDE : many > SEGMI_NUM_CU ? MANY : FEW;
 }
-#define NS_LAUNCH(bt, kernel128, kernel64, grid, ...)                                                          \
-    do {                                                                                                       \
-        if ((bt) == 128) hipLaunchKernelGGL(kernel128, dim3(grid), dim3(256), 0, st, __VA_ARGS__);             \
-        else hipLaunchKernelGGL(kernel64, dim3(grid), dim3(256), 0, st, __VA_ARGS__);                          \
+#define NS_LAUNCH(config, kernel, grid, ...)                                                                               \
+    do {                                                                                                                   \
+        if ((config) == WIDE) hipLaunchKernelGGL((kernel(Wide)), dim3(grid), dim3(256), 0, st, __VA_ARGS__);               \
+        else if ((config) == MANY) hipLaunchKernelGGL((kernel(Many)), dim3(grid), dim3(256), 0, st, __VA_ARGS__);          \
+        else hipLaunchKernelGGL((kernel(Few)), dim3(grid), dim3(256), 0, st, __VA_ARGS__);                                 \
     } while (0)
+#define NS_GRAM(C) ns_gram<C>
+#define NS_POLY(C) ns_square_product<C, true>
+#define NS_SQUARE(C) ns_square_product<C, false>
+#define NS_APPLY(C) ns_apply<C>
+#define NS_FINISH(C) ns_finish<C, MUON>
 
-// runs of a Gram product: enough workgroups to fill the chip, no run shorter than 16 lines
 struct GramPlan {
+    Config config;
     int bt;
     unsigned run;
 };
 GramPlan gram_plan(const Shape* s, int count) {
-    GramPlan best{64, 0};
     double work128 = 0.0, work64 = 0.0;
     for (int i = 0; i < count; ++i) {
         work128 += (double)low_tiles(s[i].m, 128) * (pad64(s[i].n) / LINE_K);
         work64 += (double)low_tiles(s[i].m, 64) * (pad64(s[i].n) / LINE_K);
     }
-    best.bt = work128 / 16.0 >= 512.0 ? 128 : 64;
-    const double run = std::ceil((best.bt == 128 ? work128 / 1024.0 : work64 / 2048.0) / 4.0) * 4.0;
-    best.run = run < 16.0 ? 16u : (unsigned)run;         // whole steps of a tile
-    return best;
+    GramPlan g;
+    g.config = work128 / 16.0 >= 512.0 ? WIDE : work64 / 16.0 > SEGMI_NUM_CU ? MANY : FEW;
+    g.bt = tile_of(g.config);
+    const double run = std::ceil((g.config == WIDE ? work128 / 512.0 : work64 / 1024.0) / 4.0) * 4.0;
+    g.run = run < 16.0 ? 16u : (unsigned)run;            // whole steps of a tile
+    return g;
 }
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -837,8 +862,9 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
               const Hyper& h, const Hyper* hd, hipStream_t st) {
     const Plan plan = plan_batch(shapes, count);
     const GramPlan gp = gram_plan(shapes, count);
-    const int bt_sq = tile_size(shapes, count, [](const Shape& x, int bt) { return low_tiles(x.m, bt); });
-    const int bt_big = tile_size(shapes, count, big_tiles);
+    const Config c_sq = config_of(shapes, count, [](const Shape& x, int bt) { return low_tiles(x.m, bt); });
+    const Config c_big = config_of(shapes, count, big_tiles);
+    const int bt_sq = tile_of(c_sq), bt_big = tile_of(c_big);
     Batch sq, big;
     GramBatch gram;
     src.ws = dst.ws = sq.ws = big.ws = gram.ws = ws + plan.mats_at;
@@ -888,12 +914,13 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
         const int len = segment_length(wide, seg, left);
         double sa = Bounds::scale_for(s * s);
         gram.scale = (float)(sa / (sx * sx));
-        NS_LAUNCH(gp.bt, ns_gram<128>, ns_gram<64>, g_gram, gram);
-        NS_LAUNCH(gp.bt, ns_gram_reduce<128>, ns_gram_reduce<64>, g_red, gram);
+        NS_LAUNCH(gp.config, NS_GRAM, g_gram, gram);
+        if (gp.bt == 128) hipLaunchKernelGGL((ns_gram_reduce<128>), dim3(g_red), dim3(256), 0, st, gram);
+        else hipLaunchKernelGGL((ns_gram_reduce<64>), dim3(g_red), dim3(256), 0, st, gram);
         const auto product = [&](int l, int r, int out, double so, double sl, double sr) { return Product{l, r, out, (float)(so / (sl * sr)), 0.f, 0.f}; };
         const auto square = [&](int out, double so, double ident) {      // out = ident I + b A + c A^2
             const Product pr{A, A, out, (float)(f.c * so / (sa * sa)), (float)(ident * so), (float)(f.b * so / sa)};
-            NS_LAUNCH(bt_sq, (ns_square_product<128, true>), (ns_square_product<64, true>), g_sq, sq, pr);
+            NS_LAUNCH(c_sq, NS_POLY, g_sq, sq, pr);
         };
         const double s1 = f.max_p(s) * SLACK;            // bound after the segment's first step
         double sp, alpha = 0.0;
@@ -908,12 +935,12 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
             const double bq0 = f.max_q(s) * SLACK, bq1 = f.max_q(s1) * SLACK;
             const double sq0 = Bounds::scale_for(bq0), sw = Bounds::scale_for(s * s1), san = Bounds::scale_for(s1 * s1), sq1 = Bounds::scale_for(bq1);
             square(P0, sq0, f.a);
-            NS_LAUNCH(bt_sq, (ns_square_product<128, false>), (ns_square_product<64, false>), g_sq, sq, product(P0, A, W, sw, sq0, sa));
-            NS_LAUNCH(bt_sq, (ns_square_product<128, false>), (ns_square_product<64, false>), g_sq, sq, product(W, P0, A, san, sw, sq0));
+            NS_LAUNCH(c_sq, NS_SQUARE, g_sq, sq, product(P0, A, W, sw, sq0, sa));
+            NS_LAUNCH(c_sq, NS_SQUARE, g_sq, sq, product(W, P0, A, san, sw, sq0));
             sa = san;
             square(Q, sq1, f.a);
             sp = Bounds::scale_for(bq0 * bq1);
-            NS_LAUNCH(bt_sq, (ns_square_product<128, false>), (ns_square_product<64, false>), g_sq, sq, product(P0, Q, P1, sp, sq0, sq1));
+            NS_LAUNCH(c_sq, NS_SQUARE, g_sq, sq, product(P0, Q, P1, sp, sq0, sq1));
             p = P1;
             s = f.max_p(s1) * SLACK;
         }
@@ -921,7 +948,7 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
         if (left > 0) {
             const double nsx = Bounds::scale_for(s);
             const int tout = tin == T0 ? T1 : T0;
-            NS_LAUNCH(bt_big, ns_apply<128>, ns_apply<64>, g_big, big, p, tin, tout, (float)(nsx / (sp * sx)), (float)(alpha * nsx / sx));
+            NS_LAUNCH(c_big, NS_APPLY, g_big, big, p, tin, tout, (float)(nsx / (sp * sx)), (float)(alpha * nsx / sx));
             tin = tout;
             sx = nsx;
         } else {
@@ -929,7 +956,7 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
             dst.tin = tin;
             dst.scale = (float)(1.0 / (sp * sx));
             dst.alpha = (float)(alpha / sx);
-            NS_LAUNCH(bt_big, (ns_finish<128, MUON>), (ns_finish<64, MUON>), g_big, dst, h, hd);
+            NS_LAUNCH(c_big, NS_FINISH, g_big, dst, h, hd);
         }
     }
     return segmi_launch_status();
@@ -946,19 +973,21 @@ Shape shape_of(int rows, int cols, bool cols_inner) {
 
 Shape shape_of(const segmi_ns_matrix& a) { return shape_of(a.rows, a.cols, a.src_cs == 1 || a.src_rs != 1); }
 
-// The matrices of a call in batches of one class (wide or not) and at most BATCH each: f(indices, how many) in order, until it
-// returns something other than SEGMI_OK.  Batches run one after the other and share the workspace.
+// The matrices of a call in batches of one class (wide or not) and at most BATCH each, those with the longest sums first (what is
+// started last should be short): f(indices, how many) in order, until it returns something other than SEGMI_OK.  Batches run one
+// after the other and share the workspace.
 template <typename M, typename F>
 int for_batches(const M* mats, int count, F f) {
+    const auto side = [&](int i) { return mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols; };
+    std::vector<int> order(count);
     for (int wide = 0; wide < 2; ++wide) {
-        int index[BATCH], k = 0;
-        for (int i = 0; i < count; ++i) {
-            if (is_wide(mats[i].rows, mats[i].cols) == (wide != 0)) index[k++] = i;
-            if (k == BATCH || (i == count - 1 && k)) {
-                const int rc = f(index, k);
-                if (rc != SEGMI_OK) return rc;
-                k = 0;
-            }
+        int k = 0;
+        for (int i = 0; i < count; ++i)
+            if (is_wide(mats[i].rows, mats[i].cols) == (wide != 0)) order[k++] = i;
+        std::stable_sort(order.begin(), order.begin() + k, [&](int a, int b) { return side(a) > side(b); });
+        for (int at = 0; at < k; at += BATCH) {
+            const int rc = f(order.data() + at, k - at < BATCH ? k - at : BATCH);
+            if (rc != SEGMI_OK) return rc;
         }
     }
     return SEGMI_OK;
