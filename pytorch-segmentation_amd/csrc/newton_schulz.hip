@@ -36,6 +36,7 @@ namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int BATCH = 48;            // matrices per launch: their descriptors travel as kernel arguments (< 4 KiB)
 constexpr int MAX_GROUPS = 8;
@@ -71,9 +72,18 @@ __device__ __forceinline__ int find_item(const B& b, unsigned wg) {
     return __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(first <= wg)) - 1);
 }
 
+// hi = v rounded, lo = the rest rounded.  The empty statement makes v one fp32 number: the compiler may otherwise round the expression
+// behind v straight to fp16 for hi, in one step, and take the rest from v, rounded in two, which now and then is a neighbour's.
 __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
+    asm("" : "+v"(v));
     hi = (_Float16)v;
-    lo = (_Float16)(v - (float)hi);
+    lo = (_Float16)__builtin_fmaf((float)hi, -1.f, v);
+}
+__device__ __forceinline__ float join(_Float16 hi, _Float16 lo) { return __builtin_fmaf((float)lo, 1.f, (float)hi); }
+__device__ __forceinline__ unsigned pair_word(float v) {
+    _Float16 h, l;
+    split(v, h, l);
+    return __builtin_bit_cast(unsigned, f16x2{h, l});
 }
 // where value k of a row lies
 __device__ __forceinline__ size_t at_line(unsigned lines, unsigned row, unsigned k) {
@@ -104,7 +114,7 @@ __device__ __forceinline__ void load4(const char* buf, unsigned lines, unsigned 
     const char* p = buf + at_line(lines, row, k);
     const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + LINE / 2);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) v[x] = (float)hi[x] + (float)lo[x];
+    for (int x = 0; x < 4; ++x) v[x] = join(hi[x], lo[x]);
 }
 
 // ------------------------------------------------------------------------------------------------ reading the updates
@@ -137,8 +147,8 @@ struct Hyper {
 __device__ __forceinline__ float bf16_to_f32(unsigned short u) { return __uint_as_float((unsigned)u << 16); }
 __device__ __forceinline__ unsigned short f32_to_bf16(float f) {
     const unsigned u = __float_as_uint(f);
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (unsigned short)((u >> 16) | 0x40u);        // NaN stays NaN
-    return (unsigned short)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);                       // round to nearest, ties to even
+    const unsigned nearest = (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;                        // ties to even
+    return (unsigned short)(f != f ? (u >> 16) | 0x40u : nearest);                          // NaN stays NaN
 }
 
 __device__ __forceinline__ float source_at(const Source& s, long off) {
@@ -433,9 +443,7 @@ struct Tile {
     // Turning a tile round in LDS: a lane holds runs of rows of one column, a row's line wants runs of columns.  `park` keeps the pair
     // of a value, `store_rows` writes all parked rows, 16 B a lane.  Pitch: 4 rows apart is 32 banks apart.
     __device__ __forceinline__ static void park(char* smem, int row, int col, float v) {
-        _Float16 h, l;
-        split(v, h, l);
-        reinterpret_cast<unsigned*>(smem)[row * PITCH + col] = __builtin_bit_cast(unsigned short, h) | (unsigned)__builtin_bit_cast(unsigned short, l) << 16;
+        reinterpret_cast<unsigned*>(smem)[row * PITCH + col] = pair_word(v);
     }
     __device__ __forceinline__ static void store_rows(const char* smem, char* out, unsigned lines, unsigned r0, unsigned c0, unsigned rows, unsigned cols) {
         __syncthreads();
@@ -708,6 +716,299 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_finish(TargetBatch b, Hyper
     });
 }
 
+// ------------------------------------------------------------------------------------------------ small matrices
+// One workgroup does the whole iteration of a matrix whose X fits its registers: m <= 32 R rows, n <= 256 G columns; one launch instead of 22.
+// Wave w of 8 owns the 32-column slices w, w + 8, ...; a lane holds one column of each, in the order of a matrix
+// instruction's result (rows 8 e + 4 (lane / 32) + 0 .. 3 of each 32).  Steps one by one:
+//     A = X X^T    each wave turns its slices in LDS (words hi | lo << 16) and sums its columns' products; the 8 sums are added in order
+//     Q = b A + c A^2
+//     X <- a X + Q X    X goes into the instruction as it lies in the registers: the sum over rows may run in any order, so Q's words
+//                       are read in the order in which a lane holds the rows
+// Bound by latency: 64 x 576 is 25 MFLOP a step on one CU (2.7 us at its peak rate) plus four barriers.
+struct SmallItem {
+    const void* src;                 // MUON: the gradient
+    void* dst;                       // MUON: the parameter
+    float* mom;
+    long si, sj, di, dj;             // strides of X's rows and columns in src (and mom), and in dst
+    int m, n;
+    float factor;
+    int dtype, group;
+    unsigned src_bytes, dst_bytes;   // up to the last element
+};
+struct SmallStep {
+    float gram, quad, lin, apply;    // fp32 sums to the next stored scale; X <- a X + Q X keeps X's scale `apply` folded in
+    float alpha;
+};
+constexpr int SMALL_BATCH = 32;
+struct SmallBatch {
+    double eps;
+    float scale, unscale;            // of the first X, and of the last one's inverse
+    int steps, nesterov;
+    SmallStep step[SEGMI_NS_MAX_STEPS];
+    SmallItem item[SMALL_BATCH];
+};
+
+__device__ __forceinline__ float word_value(unsigned w) {
+    const f16x2 p = __builtin_bit_cast(f16x2, w);
+    return join(p[0], p[1]);
+}
+struct PairFrag {
+    f16x8 hi, lo;
+    __device__ __forceinline__ void from_words(uint4 p, uint4 q) {
+        const uint4 h = make_uint4(__builtin_amdgcn_perm(p.y, p.x, 0x05040100u), __builtin_amdgcn_perm(p.w, p.z, 0x05040100u),
+                                   __builtin_amdgcn_perm(q.y, q.x, 0x05040100u), __builtin_amdgcn_perm(q.w, q.z, 0x05040100u));
+        const uint4 l = make_uint4(__builtin_amdgcn_perm(p.y, p.x, 0x07060302u), __builtin_amdgcn_perm(p.w, p.z, 0x07060302u),
+                                   __builtin_amdgcn_perm(q.y, q.x, 0x07060302u), __builtin_amdgcn_perm(q.w, q.z, 0x07060302u));
+        hi = __builtin_bit_cast(f16x8, h);
+        lo = __builtin_bit_cast(f16x8, l);
+    }
+};
+__device__ __forceinline__ void pair_product(const PairFrag& l, const PairFrag& r, f32x16& acc, f32x16& mix) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(l.hi, r.hi, acc, 0, 0, 0);
+    mix = __builtin_amdgcn_mfma_f32_32x32x16_f16(l.lo, r.hi, mix, 0, 0, 0);
+    mix = __builtin_amdgcn_mfma_f32_32x32x16_f16(l.hi, r.lo, mix, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) z[x] = 0.f;
+    return z;
+}
+
+template <int R, int G, bool MUON>
+__global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const Hyper* __restrict__ hd) {
+    constexpr int SUBS = R * (R + 1) / 2;                // 32 x 32 subtiles on and below the diagonal
+    constexpr int XP = 36, AP = 32 * R + 4;              // row pitches in words: ds_read_b128 of 16 rows covers all 64 banks
+    __shared__ __attribute__((aligned(16))) union {
+        unsigned x[8][32 * R][XP];                       // a wave's slice, turned
+        float4 part[8][SUBS][4][64];                     // the waves' sums
+    } u;
+    __shared__ __attribute__((aligned(16))) unsigned a_words[32 * R][AP];
+    __shared__ __attribute__((aligned(16))) unsigned q_words[32 * R][AP];
+    __shared__ double red[8];
+    const SmallItem& s = b.item[blockIdx.x];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int m = s.m, n = s.n;
+    const int slices = (n + 31) / 32;
+    const float mu = MUON ? (hd ? hd->mom[s.group] : h.mom[s.group]) : 0.f;
+    const bool nest = MUON && b.nesterov;
+
+    // An element's byte offset is a lane's part (column, half of the rows) plus a uniform part (the row in the half): the instruction
+    // adds the two.  A lane outside the matrix gets an offset beyond the buffer, which reads as 0 and drops what is written.
+    const unsigned size = s.dtype ? 2 : 4;
+    const auto lane_offset = [&](int g, long si, long sj) {
+        const int j = (g * 8 + wave) * 32 + col;
+        return j < n ? ((unsigned)j * (unsigned)sj + 4u * half * (unsigned)si) * size : 0xFFFFFFFFu;
+    };
+    // f(r, e, lane's part, uniform part) for the elements of a slice; the uniform part never leaves the buffer
+    const auto each = [&](unsigned at, long si, auto f) {
+        int rows = m - 4 * half;                         // the comparisons are made anew each time: kept, their masks would fill the registers
+        asm volatile("" : "+v"(rows));
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const unsigned i = 32 * r + 8 * (e >> 2) + (e & 3);
+                f(r, e, (int)i < rows ? at : 0xFFFFFFFFu, (int)i < m ? i * (unsigned)si * size : 0u);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(s.src), 0, s.src_bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t mom = __builtin_amdgcn_make_buffer_rsrc(s.mom, 0, MUON ? s.src_bytes : 0, 0x00020000);
+    const __amdgpu_buffer_rsrc_t dst = __builtin_amdgcn_make_buffer_rsrc(s.dst, 0, s.dst_bytes, 0x00020000);
+    const auto load = [](__amdgpu_buffer_rsrc_t b, unsigned lane_part, unsigned part) {
+        return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, lane_part, part, 0));
+    };
+
+    float x[G][R][16];
+    unsigned w[G][R][16];                                // X as pairs, from the first step on
+    double sum = 0.0;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const unsigned at = lane_offset(g, s.si, s.sj);
+        if (s.dtype)
+            each(at, s.si, [&](int r, int e, unsigned lp, unsigned up) { x[g][r][e] = bf16_to_f32(__builtin_amdgcn_raw_buffer_load_b16(src, lp, up, 0)); });
+        else
+            each(at, s.si, [&](int r, int e, unsigned lp, unsigned up) { x[g][r][e] = load(src, lp, up); });
+    }
+    if (MUON)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const unsigned at = lane_offset(g, s.si, s.sj);
+            float v[R][16];                              // all loads first: behind a store they would wait for it
+            each(at, s.si, [&](int r, int e, unsigned lp, unsigned up) { v[r][e] = fmaf(mu, load(mom, lp, up), x[g][r][e]); });
+            each(at, s.si, [&](int r, int e, unsigned lp, unsigned up) {
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[r][e]), mom, lp, up, 0);
+                x[g][r][e] = nest ? fmaf(mu, v[r][e], x[g][r][e]) : v[r][e];
+            });
+        }
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum = fma((double)x[g][r][e], (double)x[g][r][e], sum);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    const double norm = sqrt(((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7])));
+    int power;                                           // the factor may lie outside fp32's range: a number in [1/2, 1) and a power of two
+    const float factor = (float)frexp((double)b.scale / (norm <= b.eps ? b.eps : norm), &power);      // (a NaN norm stays)
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[g][r][e] = pair_word(__builtin_amdgcn_ldexpf(x[g][r][e] * factor, power));
+
+    for (int step = 0; step < b.steps; ++step) {
+        const SmallStep k = b.step[step];
+        {   // A = X X^T
+            f32x16 acc[SUBS], mix[SUBS];
+#pragma unroll
+            for (int t = 0; t < SUBS; ++t) acc[t] = mix[t] = zero16();
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                if (g * 8 + wave >= slices) continue;
+                // (a wave's own LDS: its reads follow its writes in order, no barrier)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) u.x[wave][32 * r + 8 * (e >> 2) + 4 * half + (e & 3)][col] = w[g][r][e];
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    PairFrag f[R];
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const uint4* const p = reinterpret_cast<const uint4*>(&u.x[wave][32 * r + col][ks * 16 + half * 8]);
+                        f[r].from_words(p[0], p[1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < R; ++i)
+#pragma unroll
+                        for (int j = 0; j <= i; ++j) pair_product(f[i], f[j], acc[i * (i + 1) / 2 + j], mix[i * (i + 1) / 2 + j]);
+                    __builtin_amdgcn_sched_barrier(0);   // (slices and steps one after the other: all at once do not fit the registers)
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    u.part[wave][t][e][lane] = make_float4(acc[t][4 * e] + mix[t][4 * e], acc[t][4 * e + 1] + mix[t][4 * e + 1],
+                                                           acc[t][4 * e + 2] + mix[t][4 * e + 2], acc[t][4 * e + 3] + mix[t][4 * e + 3]);
+            __syncthreads();
+            for (int p = tid; p < SUBS * 256; p += 512) {
+                const int t = p >> 8, e = (p >> 6) & 3, l = p & 63;
+                float4 v = u.part[0][t][e][l];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) {
+                    const float4 q = u.part[i][t][e][l];
+                    v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+                }
+                const int ti = t == 0 ? 0 : 1, tj = t == 2 ? 1 : 0;
+                const int row = 32 * ti + 8 * e + 4 * (l >> 5), c = 32 * tj + (l & 31);
+                const uint4 a = make_uint4(pair_word(v.x * k.gram), pair_word(v.y * k.gram), pair_word(v.z * k.gram), pair_word(v.w * k.gram));
+                *reinterpret_cast<uint4*>(&a_words[c][row]) = a;
+                if (ti != tj) {
+                    a_words[row][c] = a.x;
+                    a_words[row + 1][c] = a.y;
+                    a_words[row + 2][c] = a.z;
+                    a_words[row + 3][c] = a.w;
+                }
+            }
+        }
+        __syncthreads();
+        if (wave < SUBS) {   // Q = b A + c A^2, a wave per subtile
+            const int ti = wave == 0 ? 0 : 1, tj = wave == 2 ? 1 : 0;
+            f32x16 acc = zero16(), mix = zero16();
+#pragma unroll
+            for (int ks = 0; ks < 2 * R; ++ks) {
+                PairFrag l, r;
+                const uint4* const p = reinterpret_cast<const uint4*>(&a_words[32 * ti + col][ks * 16 + half * 8]);
+                const uint4* const q = reinterpret_cast<const uint4*>(&a_words[32 * tj + col][ks * 16 + half * 8]);
+                l.from_words(p[0], p[1]);
+                r.from_words(q[0], q[1]);
+                pair_product(l, r, acc, mix);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = 32 * ti + 8 * e + 4 * half, c = 32 * tj + col;
+                const uint4 av = *reinterpret_cast<const uint4*>(&a_words[c][row]);
+                const unsigned w0 = pair_word(fmaf(k.lin, word_value(av.x), (acc[4 * e] + mix[4 * e]) * k.quad));
+                const unsigned w1 = pair_word(fmaf(k.lin, word_value(av.y), (acc[4 * e + 1] + mix[4 * e + 1]) * k.quad));
+                const unsigned w2 = pair_word(fmaf(k.lin, word_value(av.z), (acc[4 * e + 2] + mix[4 * e + 2]) * k.quad));
+                const unsigned w3 = pair_word(fmaf(k.lin, word_value(av.w), (acc[4 * e + 3] + mix[4 * e + 3]) * k.quad));
+                *reinterpret_cast<uint4*>(&q_words[c][row]) = make_uint4(w0, w1, w2, w3);
+                if (ti != tj) {
+                    q_words[row][c] = w0;
+                    q_words[row + 1][c] = w1;
+                    q_words[row + 2][c] = w2;
+                    q_words[row + 3][c] = w3;
+                }
+            }
+        }
+        __syncthreads();
+        // X <- a X + Q X
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            if (g * 8 + wave >= slices) continue;
+            f32x16 acc[R], mix[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[r] = mix[r] = zero16();
+#pragma unroll
+            for (int t = 0; t < 2 * R; ++t) {            // rows 16 t .. 16 t + 15 of X
+                PairFrag xf;
+                const unsigned* const v = &w[g][t >> 1][8 * (t & 1)];
+                xf.from_words(make_uint4(v[0], v[1], v[2], v[3]), make_uint4(v[4], v[5], v[6], v[7]));
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    PairFrag qf;
+                    qf.from_words(*reinterpret_cast<const uint4*>(&q_words[32 * r + col][16 * t + 4 * half]),
+                                  *reinterpret_cast<const uint4*>(&q_words[32 * r + col][16 * t + 8 + 4 * half]));
+                    pair_product(qf, xf, acc[r], mix[r]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) w[g][r][e] = pair_word(fmaf(k.alpha, word_value(w[g][r][e]), (acc[r][e] + mix[r][e]) * k.apply));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // (the next step's first barrier lies behind its turning of X, which touches neither A nor Q)
+    }
+
+    float keep = 1.f, rate = 0.f;
+    if (MUON) {
+        const float lr = hd ? hd->lr[s.group] : h.lr[s.group], wd = hd ? hd->wd[s.group] : h.wd[s.group];
+        keep = 1.f - lr * wd;
+        rate = lr * s.factor;
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const unsigned at = lane_offset(g, s.di, s.dj);
+        if (MUON) {
+            float v[R][16];
+            each(at, s.di, [&](int r, int e, unsigned lp, unsigned up) { v[r][e] = load(dst, lp, up); });
+            each(at, s.di, [&](int r, int e, unsigned lp, unsigned up) {
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(fmaf(-rate, word_value(w[g][r][e]) * b.unscale, v[r][e] * keep)), dst, lp, up, 0);
+            });
+        } else if (s.dtype) {
+            each(at, s.di, [&](int r, int e, unsigned lp, unsigned up) {
+                __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(word_value(w[g][r][e]) * b.unscale), dst, lp, up, 0);
+            });
+        } else {
+            each(at, s.di, [&](int r, int e, unsigned lp, unsigned up) {
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(word_value(w[g][r][e]) * b.unscale), dst, lp, up, 0);
+            });
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 // Largest value of |f| on [0, s] for the polynomials of the iteration, and the power-of-two scale that keeps such entries below 2^15
 // (fp16 ends at 65504; a matrix's entries are bounded by its spectral norm).
@@ -762,10 +1063,24 @@ constexpr double MAX_BOUND = 4096.0;                     // coefficients whose i
 // Steps between Gram products: one by one for matrices of nearly square shape and for small ones, else 2, 1, 2, 1, ... (see the head
 // of this file; below 65 rows the sums are so short that fp32 rounds hardly at all, and 2 + 1 + 2 came out at up to 2.2 times its distance)
 int segment_length(bool wide, int index, int left) { return wide && (index & 1) == 0 && left >= 2 ? 2 : 1; }
-bool is_wide(int rows, int cols) {
+enum Class { SMALL_1_1, SMALL_1_3, SMALL_1_9, SMALL_2_1, SMALL_2_3, SQUARE, WIDE_MATRIX, CLASSES };
+bool is_wide(int m, int n) { return m > 64 && n / 2 >= m; }
+// `span`: bytes from the first to behind the last element; ns_small<R, G> addresses with 32 bits
+Class class_of(int rows, int cols, size_t span) {
     const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-    return m > 64 && n / 2 >= m;
+    if (span < ((size_t)1 << 31)) {
+        if (m <= 32 && n <= 2304) return n <= 256 ? SMALL_1_1 : n <= 768 ? SMALL_1_3 : SMALL_1_9;
+        if (m <= 64 && n <= 768) return n <= 256 ? SMALL_2_1 : SMALL_2_3;
+    }
+    return is_wide(m, n) ? WIDE_MATRIX : SQUARE;
 }
+size_t span_of(const segmi_ns_matrix& a) {
+    const auto end = [&](long rs, long cs) { return ((size_t)(a.rows - 1) * rs + (size_t)(a.cols - 1) * cs + 1) * (a.dtype ? 2 : 4); };
+    return std::max(end(a.src_rs, a.src_cs), end(a.dst_rs, a.dst_cs));
+}
+size_t span_of(const segmi_muon_matrix& a) { return (size_t)a.rows * a.cols * 4; }
+template <typename M>
+Class class_of(const M& a) { return class_of(a.rows, a.cols, span_of(a)); }
 
 bool iteration_ok(const Bounds& f, int steps) {
     double s = SLACK;
@@ -962,6 +1277,29 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
     return segmi_launch_status();
 }
 
+// `b` carries the callers' pointers; the steps' scales are filled in here
+template <bool MUON>
+int run_small(Class c, SmallBatch& b, int count, const Bounds& f, int steps, const Hyper& h, const Hyper* hd, hipStream_t st) {
+    double s = SLACK, sx = Bounds::scale_for(s);
+    b.scale = (float)sx;
+    b.steps = steps;
+    for (int i = 0; i < steps; ++i) {
+        const double sa = Bounds::scale_for(s * s), sq = Bounds::scale_for(f.max_r(s) * SLACK);
+        s = f.max_p(s) * SLACK;
+        const double nsx = Bounds::scale_for(s);
+        b.step[i] = SmallStep{(float)(sa / (sx * sx)), (float)(f.c * sq / (sa * sa)), (float)(f.b * sq / sa), (float)(nsx / (sq * sx)), (float)(f.a * nsx / sx)};
+        sx = nsx;
+    }
+    b.unscale = (float)(1.0 / sx);
+    const dim3 grid(count), threads(512);
+    if (c == SMALL_1_1) hipLaunchKernelGGL((ns_small<1, 1, MUON>), grid, threads, 0, st, b, h, hd);
+    else if (c == SMALL_1_3) hipLaunchKernelGGL((ns_small<1, 3, MUON>), grid, threads, 0, st, b, h, hd);
+    else if (c == SMALL_1_9) hipLaunchKernelGGL((ns_small<1, 9, MUON>), grid, threads, 0, st, b, h, hd);
+    else if (c == SMALL_2_1) hipLaunchKernelGGL((ns_small<2, 1, MUON>), grid, threads, 0, st, b, h, hd);
+    else hipLaunchKernelGGL((ns_small<2, 3, MUON>), grid, threads, 0, st, b, h, hd);
+    return segmi_launch_status();
+}
+
 bool shape_ok(int rows, int cols) {
     return rows > 0 && cols > 0 && big_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows) < ((size_t)1 << 32);
 }
@@ -973,20 +1311,21 @@ Shape shape_of(int rows, int cols, bool cols_inner) {
 
 Shape shape_of(const segmi_ns_matrix& a) { return shape_of(a.rows, a.cols, a.src_cs == 1 || a.src_rs != 1); }
 
-// The matrices of a call in batches of one class (wide or not) and at most BATCH each, those with the longest sums first (what is
-// started last should be short): f(indices, how many) in order, until it returns something other than SEGMI_OK.  Batches run one
-// after the other and share the workspace.
+// The matrices of a call in batches of one class, those with the longest sums first (what is started last should be short):
+// f(class, indices, how many) in order, until it returns something other than SEGMI_OK.  Batches run one after the other and share
+// the workspace.
 template <typename M, typename F>
 int for_batches(const M* mats, int count, F f) {
     const auto side = [&](int i) { return mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols; };
     std::vector<int> order(count);
-    for (int wide = 0; wide < 2; ++wide) {
+    for (int c = 0; c < CLASSES; ++c) {
         int k = 0;
         for (int i = 0; i < count; ++i)
-            if (is_wide(mats[i].rows, mats[i].cols) == (wide != 0)) order[k++] = i;
+            if (class_of(mats[i]) == c) order[k++] = i;
         std::stable_sort(order.begin(), order.begin() + k, [&](int a, int b) { return side(a) > side(b); });
-        for (int at = 0; at < k; at += BATCH) {
-            const int rc = f(order.data() + at, k - at < BATCH ? k - at : BATCH);
+        const int most = c < SQUARE ? SMALL_BATCH : BATCH;
+        for (int at = 0; at < k; at += most) {
+            const int rc = f((Class)c, order.data() + at, k - at < most ? k - at : most);
             if (rc != SEGMI_OK) return rc;
         }
     }
@@ -995,8 +1334,9 @@ int for_batches(const M* mats, int count, F f) {
 
 template <typename M, typename F>
 size_t workspace_of(const M* mats, int count, F shape) {
-    size_t most = 0;
-    for_batches(mats, count, [&](const int* index, int k) {
+    size_t most = 256;                                   // (small matrices need none; 0 means refused)
+    for_batches(mats, count, [&](Class c, const int* index, int k) {
+        if (c < SQUARE) return (int)SEGMI_OK;
         Shape s[BATCH];
         for (int i = 0; i < k; ++i) s[i] = shape(mats[index[i]]);
         const Plan p = plan_batch(s, k);
@@ -1032,7 +1372,18 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
     if ((size_t)workspace & 255) return SEGMI_ERR_ALIGN;
     if (workspace_bytes < segmi_ns_workspace(mats_host, count)) return SEGMI_ERR_WORKSPACE;
     const Bounds f{coefficients_host[0], coefficients_host[1], coefficients_host[2]};
-    return for_batches(mats_host, count, [&](const int* index, int k) {
+    return for_batches(mats_host, count, [&](Class cls, const int* index, int k) {
+        if (cls < SQUARE) {
+            SmallBatch b{};
+            b.eps = eps;
+            for (int i = 0; i < k; ++i) {
+                const segmi_ns_matrix& a = mats_host[index[i]];
+                const bool wide = a.rows <= a.cols;
+                b.item[i] = SmallItem{a.src, a.dst, nullptr, wide ? a.src_rs : a.src_cs, wide ? a.src_cs : a.src_rs, wide ? a.dst_rs : a.dst_cs,
+                                      wide ? a.dst_cs : a.dst_rs, wide ? a.rows : a.cols, wide ? a.cols : a.rows, 0.f, a.dtype, 0, (unsigned)span_of(a), (unsigned)span_of(a)};
+            }
+            return run_small<false>(cls, b, k, f, steps, Hyper{}, nullptr, (hipStream_t)stream);
+        }
         Shape shapes[BATCH];
         SourceBatch src{};
         TargetBatch dst{};
@@ -1089,7 +1440,20 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
             h.wd[i] = weight_decay_host[i];
             h.mom[i] = momentum_host[i];
         }
-    return for_batches(mats_host, count, [&](const int* index, int k) {
+    return for_batches(mats_host, count, [&](Class cls, const int* index, int k) {
+        if (cls < SQUARE) {
+            SmallBatch b{};
+            b.eps = eps;
+            b.nesterov = nesterov;
+            for (int i = 0; i < k; ++i) {
+                const segmi_muon_matrix& a = mats_host[index[i]];
+                const bool wide = a.rows <= a.cols;
+                const long si = wide ? a.cols : 1, sj = wide ? 1 : a.cols;
+                b.item[i] = SmallItem{a.grad, a.param, a.momentum, si, sj, si, sj, wide ? a.rows : a.cols, wide ? a.cols : a.rows, a.factor, 0, a.group,
+                                      (unsigned)span_of(a), (unsigned)span_of(a)};
+            }
+            return run_small<true>(cls, b, k, f, steps, h, reinterpret_cast<const Hyper*>(hyper_dev), (hipStream_t)stream);
+        }
         Shape shapes[BATCH];
         SourceBatch src{};
         TargetBatch dst{};
