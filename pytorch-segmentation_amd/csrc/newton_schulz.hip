@@ -748,10 +748,28 @@ struct SmallBatch {
     SmallItem item[SMALL_BATCH];
 };
 
-__device__ __forceinline__ float word_value(unsigned w) {
-    const f16x2 p = __builtin_bit_cast(f16x2, w);
-    return join(p[0], p[1]);
-}
+// two values' pairs: hi of both in one register, lo of both in another; the mixed-precision instructions take the halves as they lie
+struct Pair2 {
+    unsigned hi, lo;
+    __device__ __forceinline__ void set(float a, float b) {
+        asm("" : "+v"(a), "+v"(b));                      // as in `split`
+        hi = __builtin_bit_cast(unsigned, f16x2{(_Float16)a, (_Float16)b});
+        asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]\n\t"
+            "v_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=&v"(lo) : "v"(hi), "v"(a), "v"(b));
+    }
+    // f * value
+    __device__ __forceinline__ float times(int which, float f) const {
+        float v;
+        if (which)
+            asm("v_fma_mix_f32 %0, %1, %3, 0 op_sel:[1,0,0] op_sel_hi:[1,0,0]\n\t"
+                "v_fma_mix_f32 %0, %2, %3, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=&v"(v) : "v"(lo), "v"(hi), "v"(f));
+        else
+            asm("v_fma_mix_f32 %0, %1, %3, 0 op_sel:[0,0,0] op_sel_hi:[1,0,0]\n\t"
+                "v_fma_mix_f32 %0, %2, %3, %0 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=&v"(v) : "v"(lo), "v"(hi), "v"(f));
+        return v;
+    }
+    __device__ __forceinline__ unsigned word(int which) const { return __builtin_amdgcn_perm(lo, hi, which ? 0x07060302u : 0x05040100u); }
+};
 struct PairFrag {
     f16x8 hi, lo;
     __device__ __forceinline__ void from_words(uint4 p, uint4 q) {
@@ -761,6 +779,46 @@ struct PairFrag {
                                    __builtin_amdgcn_perm(q.y, q.x, 0x07060302u), __builtin_amdgcn_perm(q.w, q.z, 0x07060302u));
         hi = __builtin_bit_cast(f16x8, h);
         lo = __builtin_bit_cast(f16x8, l);
+    }
+    __device__ __forceinline__ void from_pairs(const Pair2* p) {
+        hi = __builtin_bit_cast(f16x8, make_uint4(p[0].hi, p[1].hi, p[2].hi, p[3].hi));
+        lo = __builtin_bit_cast(f16x8, make_uint4(p[0].lo, p[1].lo, p[2].lo, p[3].lo));
+    }
+};
+// a symmetric 32 R x 32 R matrix in LDS as two planes; the pitch lets ds_read_b128 of 16 rows cover all 64 banks
+template <int R>
+struct PairPlanes {
+    static constexpr int PITCH = 32 * R + 8;
+    _Float16 hi[32 * R][PITCH], lo[32 * R][PITCH];
+    // values (row .. row + 3, col), and their mirror images if `mirror`
+    __device__ __forceinline__ void store(int row, int col, const float* v, bool mirror) {
+        Pair2 p[2];
+        p[0].set(v[0], v[1]);
+        p[1].set(v[2], v[3]);
+        *reinterpret_cast<uint2*>(&hi[col][row]) = make_uint2(p[0].hi, p[1].hi);
+        *reinterpret_cast<uint2*>(&lo[col][row]) = make_uint2(p[0].lo, p[1].lo);
+        if (mirror)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                hi[row + x][col] = __builtin_bit_cast(f16x2, p[x >> 1].hi)[x & 1];
+                lo[row + x][col] = __builtin_bit_cast(f16x2, p[x >> 1].lo)[x & 1];
+            }
+    }
+    __device__ __forceinline__ void load(int row, int col, float f, float* v) const {       // f times the values
+        Pair2 p[2];
+        const uint2 h = *reinterpret_cast<const uint2*>(&hi[col][row]), l = *reinterpret_cast<const uint2*>(&lo[col][row]);
+        p[0].hi = h.x; p[1].hi = h.y; p[0].lo = l.x; p[1].lo = l.y;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = p[x >> 1].times(x & 1, f);
+    }
+    // eight values of a row from k on, and two times four
+    __device__ __forceinline__ PairFrag frag(int row, int k) const {
+        return PairFrag{*reinterpret_cast<const f16x8*>(&hi[row][k]), *reinterpret_cast<const f16x8*>(&lo[row][k])};
+    }
+    __device__ __forceinline__ PairFrag frag(int row, int k0, int k1) const {
+        const uint2 a = *reinterpret_cast<const uint2*>(&hi[row][k0]), b = *reinterpret_cast<const uint2*>(&hi[row][k1]);
+        const uint2 c = *reinterpret_cast<const uint2*>(&lo[row][k0]), d = *reinterpret_cast<const uint2*>(&lo[row][k1]);
+        return PairFrag{__builtin_bit_cast(f16x8, make_uint4(a.x, a.y, b.x, b.y)), __builtin_bit_cast(f16x8, make_uint4(c.x, c.y, d.x, d.y))};
     }
 };
 __device__ __forceinline__ void pair_product(const PairFrag& l, const PairFrag& r, f32x16& acc, f32x16& mix) {
@@ -778,19 +836,18 @@ __device__ __forceinline__ f32x16 zero16() {
 template <int R, int G, bool MUON>
 __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const Hyper* __restrict__ hd) {
     constexpr int SUBS = R * (R + 1) / 2;                // 32 x 32 subtiles on and below the diagonal
-    constexpr int XP = 36, AP = 32 * R + 4;              // row pitches in words: ds_read_b128 of 16 rows covers all 64 banks
+    constexpr int XP = 36;                               // row pitch in words: ds_read_b128 of 16 rows covers all 64 banks
     __shared__ __attribute__((aligned(16))) union {
         unsigned x[8][32 * R][XP];                       // a wave's slice, turned
         float4 part[8][SUBS][4][64];                     // the waves' sums
     } u;
-    __shared__ __attribute__((aligned(16))) unsigned a_words[32 * R][AP];
-    __shared__ __attribute__((aligned(16))) unsigned q_words[32 * R][AP];
+    __shared__ __attribute__((aligned(16))) PairPlanes<R> A, Q;
     __shared__ double red[8];
     const SmallItem& s = b.item[blockIdx.x];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int m = s.m, n = s.n;
-    const int slices = (n + 31) / 32;
+    const int slices = (n + 31) / 32, waves = slices < 8 ? slices : 8;
     const float mu = MUON ? (hd ? hd->mom[s.group] : h.mom[s.group]) : 0.f;
     const bool nest = MUON && b.nesterov;
 
@@ -822,7 +879,7 @@ __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const 
     };
 
     float x[G][R][16];
-    unsigned w[G][R][16];                                // X as pairs, from the first step on
+    Pair2 w[G][R][8];                                    // X as pairs, from the first step on: rows 2 p, 2 p + 1 of the order above
     double sum = 0.0;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -861,7 +918,8 @@ __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const 
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) w[g][r][e] = pair_word(__builtin_amdgcn_ldexpf(x[g][r][e] * factor, power));
+            for (int p = 0; p < 8; ++p)
+                w[g][r][p].set(__builtin_amdgcn_ldexpf(x[g][r][2 * p] * factor, power), __builtin_amdgcn_ldexpf(x[g][r][2 * p + 1] * factor, power));
 
     for (int step = 0; step < b.steps; ++step) {
         const SmallStep k = b.step[step];
@@ -876,7 +934,7 @@ __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const 
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) u.x[wave][32 * r + 8 * (e >> 2) + 4 * half + (e & 3)][col] = w[g][r][e];
+                    for (int e = 0; e < 16; ++e) u.x[wave][32 * r + 8 * (e >> 2) + 4 * half + (e & 3)][col] = w[g][r][e >> 1].word(e & 1);
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
@@ -894,89 +952,91 @@ __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const 
                 }
             }
             __syncthreads();
+            if (wave < waves)
 #pragma unroll
-            for (int t = 0; t < SUBS; ++t)
+                for (int t = 0; t < SUBS; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    u.part[wave][t][e][lane] = make_float4(acc[t][4 * e] + mix[t][4 * e], acc[t][4 * e + 1] + mix[t][4 * e + 1],
+                    for (int e = 0; e < 4; ++e)
+                        u.part[wave][t][e][lane] = make_float4(acc[t][4 * e] + mix[t][4 * e], acc[t][4 * e + 1] + mix[t][4 * e + 1],
                                                            acc[t][4 * e + 2] + mix[t][4 * e + 2], acc[t][4 * e + 3] + mix[t][4 * e + 3]);
             __syncthreads();
             for (int p = tid; p < SUBS * 256; p += 512) {
                 const int t = p >> 8, e = (p >> 6) & 3, l = p & 63;
-                float4 v = u.part[0][t][e][l];
+                float4 q[8];                             // all reads first; a wave without columns counts as zeros
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[i] = u.part[i < waves ? i : 0][t][e][l];
+                float4 v = q[0];
 #pragma unroll
                 for (int i = 1; i < 8; ++i) {
-                    const float4 q = u.part[i][t][e][l];
-                    v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+                    const float in = i < waves ? 1.f : 0.f;
+                    v.x = fmaf(in, q[i].x, v.x); v.y = fmaf(in, q[i].y, v.y); v.z = fmaf(in, q[i].z, v.z); v.w = fmaf(in, q[i].w, v.w);
                 }
                 const int ti = t == 0 ? 0 : 1, tj = t == 2 ? 1 : 0;
                 const int row = 32 * ti + 8 * e + 4 * (l >> 5), c = 32 * tj + (l & 31);
-                const uint4 a = make_uint4(pair_word(v.x * k.gram), pair_word(v.y * k.gram), pair_word(v.z * k.gram), pair_word(v.w * k.gram));
-                *reinterpret_cast<uint4*>(&a_words[c][row]) = a;
-                if (ti != tj) {
-                    a_words[row][c] = a.x;
-                    a_words[row + 1][c] = a.y;
-                    a_words[row + 2][c] = a.z;
-                    a_words[row + 3][c] = a.w;
-                }
+                const float a4[4] = {v.x * k.gram, v.y * k.gram, v.z * k.gram, v.w * k.gram};
+                A.store(row, c, a4, ti != tj);
             }
         }
         __syncthreads();
         if (wave < SUBS) {   // Q = b A + c A^2, a wave per subtile
             const int ti = wave == 0 ? 0 : 1, tj = wave == 2 ? 1 : 0;
-            f32x16 acc = zero16(), mix = zero16();
+            f32x16 acc = zero16(), mix = zero16(), mix2 = zero16();
+            PairFrag l[2 * R], r[2 * R];                 // all reads first
 #pragma unroll
             for (int ks = 0; ks < 2 * R; ++ks) {
-                PairFrag l, r;
-                const uint4* const p = reinterpret_cast<const uint4*>(&a_words[32 * ti + col][ks * 16 + half * 8]);
-                const uint4* const q = reinterpret_cast<const uint4*>(&a_words[32 * tj + col][ks * 16 + half * 8]);
-                l.from_words(p[0], p[1]);
-                r.from_words(q[0], q[1]);
-                pair_product(l, r, acc, mix);
+                l[ks] = A.frag(32 * ti + col, ks * 16 + half * 8);
+                r[ks] = A.frag(32 * tj + col, ks * 16 + half * 8);
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < 2 * R; ++ks) pair_product(l[ks], r[ks], acc, ks & 1 ? mix2 : mix);
+#pragma unroll
+            for (int y = 0; y < 16; ++y) mix[y] += mix2[y];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int row = 32 * ti + 8 * e + 4 * half, c = 32 * tj + col;
-                const uint4 av = *reinterpret_cast<const uint4*>(&a_words[c][row]);
-                const unsigned w0 = pair_word(fmaf(k.lin, word_value(av.x), (acc[4 * e] + mix[4 * e]) * k.quad));
-                const unsigned w1 = pair_word(fmaf(k.lin, word_value(av.y), (acc[4 * e + 1] + mix[4 * e + 1]) * k.quad));
-                const unsigned w2 = pair_word(fmaf(k.lin, word_value(av.z), (acc[4 * e + 2] + mix[4 * e + 2]) * k.quad));
-                const unsigned w3 = pair_word(fmaf(k.lin, word_value(av.w), (acc[4 * e + 3] + mix[4 * e + 3]) * k.quad));
-                *reinterpret_cast<uint4*>(&q_words[c][row]) = make_uint4(w0, w1, w2, w3);
-                if (ti != tj) {
-                    q_words[row][c] = w0;
-                    q_words[row + 1][c] = w1;
-                    q_words[row + 2][c] = w2;
-                    q_words[row + 3][c] = w3;
-                }
+                float v[4];
+                A.load(row, c, k.lin, v);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) v[y] = fmaf(acc[4 * e + y] + mix[4 * e + y], k.quad, v[y]);
+                Q.store(row, c, v, ti != tj);
             }
         }
         __syncthreads();
-        // X <- a X + Q X
+        // X <- a X + Q X, Q's rows one block of 16 columns ahead of the products (behind the last block comes the first again)
+        PairFrag q[R];
+        const auto q_block = [&](int t) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) q[r] = Q.frag(32 * r + col, 16 * t + 4 * half, 16 * t + 8 + 4 * half);
+        };
+        q_block(0);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             if (g * 8 + wave >= slices) continue;
-            f32x16 acc[R], mix[R];
+            f32x16 acc[R];                               // (at most 64 products: no accumulator of their own for the mixed ones)
 #pragma unroll
-            for (int r = 0; r < R; ++r) acc[r] = mix[r] = zero16();
+            for (int r = 0; r < R; ++r) acc[r] = zero16();
 #pragma unroll
             for (int t = 0; t < 2 * R; ++t) {            // rows 16 t .. 16 t + 15 of X
-                PairFrag xf;
-                const unsigned* const v = &w[g][t >> 1][8 * (t & 1)];
-                xf.from_words(make_uint4(v[0], v[1], v[2], v[3]), make_uint4(v[4], v[5], v[6], v[7]));
+                PairFrag xf, now[R];
+                xf.from_pairs(&w[g][t >> 1][4 * (t & 1)]);
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    PairFrag qf;
-                    qf.from_words(*reinterpret_cast<const uint4*>(&q_words[32 * r + col][16 * t + 4 * half]),
-                                  *reinterpret_cast<const uint4*>(&q_words[32 * r + col][16 * t + 8 + 4 * half]));
-                    pair_product(qf, xf, acc[r], mix[r]);
-                }
+                for (int r = 0; r < R; ++r) now[r] = q[r];
+                q_block((t + 1) % (2 * R));
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < R; ++r) acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now[r].lo, xf.hi, acc[r], 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < R; ++r) acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now[r].hi, xf.lo, acc[r], 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < R; ++r) acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now[r].hi, xf.hi, acc[r], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) w[g][r][e] = pair_word(fmaf(k.alpha, word_value(w[g][r][e]), (acc[r][e] + mix[r][e]) * k.apply));
+                for (int p = 0; p < 8; ++p)
+                    w[g][r][p].set(fmaf(acc[r][2 * p], k.apply, w[g][r][p].times(0, k.alpha)), fmaf(acc[r][2 * p + 1], k.apply, w[g][r][p].times(1, k.alpha)));
             __builtin_amdgcn_sched_barrier(0);
         }
         // (the next step's first barrier lies behind its turning of X, which touches neither A nor Q)
@@ -995,15 +1055,15 @@ __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const 
             float v[R][16];
             each(at, s.di, [&](int r, int e, unsigned lp, unsigned up) { v[r][e] = load(dst, lp, up); });
             each(at, s.di, [&](int r, int e, unsigned lp, unsigned up) {
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(fmaf(-rate, word_value(w[g][r][e]) * b.unscale, v[r][e] * keep)), dst, lp, up, 0);
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(fmaf(-rate, w[g][r][e >> 1].times(e & 1, b.unscale), v[r][e] * keep)), dst, lp, up, 0);
             });
         } else if (s.dtype) {
             each(at, s.di, [&](int r, int e, unsigned lp, unsigned up) {
-                __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(word_value(w[g][r][e]) * b.unscale), dst, lp, up, 0);
+                __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(w[g][r][e >> 1].times(e & 1, b.unscale)), dst, lp, up, 0);
             });
         } else {
             each(at, s.di, [&](int r, int e, unsigned lp, unsigned up) {
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(word_value(w[g][r][e]) * b.unscale), dst, lp, up, 0);
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(w[g][r][e >> 1].times(e & 1, b.unscale)), dst, lp, up, 0);
             });
         }
     }
