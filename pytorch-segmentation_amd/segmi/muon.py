@@ -9,8 +9,11 @@ All three are reached through `segmi.optim`, and the two optimizers by name from
 way the reference resolves its optimizers (`base/base_trainer.py:57`).  `AdamW` in a config stays torch.optim.AdamW.
 Pointers travel as kernel arguments: no table is uploaded, gradients may move between steps, nothing waits for the GPU.
 """
+import contextlib
 import ctypes as C
 import math
+from itertools import chain
+from operator import is_, itemgetter
 
 import numpy as np
 import torch
@@ -118,6 +121,10 @@ def _same_layout(a, b):
     return a.shape == b.shape and all(sa == sb or n == 1 for sa, sb, n in zip(a.stride(), b.stride(), a.shape))
 
 
+_ptr, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
+_params = itemgetter("params")
+
+
 class _Hyper:
     """Per-group numbers in device memory (graphs): a ring of pinned slots and stream-ordered copies, as segmi.optim.SGD's."""
     RING = 8
@@ -138,6 +145,11 @@ class _Hyper:
         self.events[i].record()
 
 
+def _on(device):
+    """The device as the current one (a context manager that costs nothing where it is already)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 class _FusedOptimizer(torch.optim.Optimizer):
     """What both optimizers share: state buffers in the parameters' memory order, descriptors that are rebuilt only when a pointer
     moved, step numbers, capture."""
@@ -146,8 +158,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
         super().__init__(params, defaults)
         self.capturable = bool(capturable)
         self._hyper = None
-        self._sig = {}
-        self._desc = {}
+        self._kept = None                            # what the last step saw and the descriptors made from it, see _plan
         self._steps = self._step_of = None           # one flat tensor of step numbers; state[p]["step"] are views of it
 
     def add_param_group(self, group):
@@ -167,7 +178,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
             for key, v in st.items():
                 if isinstance(v, torch.Tensor):
                     st[key] = v.clone()
-        self._sig.clear()
+        self._kept = None
 
     def _buffer(self, p, key):
         """state[p][key] in p's own memory order; created, or re-laid once if it arrived in another (a loaded state_dict)."""
@@ -195,37 +206,65 @@ class _FusedOptimizer(torch.optim.Optimizer):
     def _device(self):
         return self.param_groups[0]["params"][0].device
 
+    def _is_matrix(self, group, p):
+        return False
+
+    def _plan(self):
+        """The step's descriptors.  They are made anew when anything they were made from is another: the parameters, which of them have
+        gradients, the groups' settings that enter them, a state tensor, any pointer or size.  (Addresses are compared, not objects alone:
+        `p.data = ...` keeps the object.)  The comparison is the host's share of a small step, so it runs over whole lists."""
+        flat = list(chain.from_iterable(map(_params, self.param_groups)))
+        grads = [p.grad for p in flat]
+        missing = [g is None for g in grads]
+        live = [g for g in grads if g is not None] if True in missing else grads
+        k = self._kept
+        if (k is not None and len(flat) == len(k["flat"]) and all(map(is_, flat, k["flat"])) and missing == k["missing"] and
+                list(map(_ptr, live)) == k["grad_ptrs"] and [live[i].stride() for i in k["deep"]] == k["strides"]):
+            held = list(chain.from_iterable(map(dict.values, k["states"])))
+            if (len(held) == len(k["held"]) and all(map(is_, held, k["held"])) and list(map(_ptr, k["tensors"])) == k["ptrs"] and
+                    list(map(_numel, flat)) == k["numels"] and [p.shape for _, p in k["members"]] == k["shapes"] and
+                    list(map(len, map(_params, self.param_groups))) == k["lengths"] and self._settings() == k["settings"]):
+                return k
+        self._kept = None
+        k = dict(mats=None, rest=None)
+        if not live:
+            return k
+        if self._device().type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("%s: a parameter, gradient or state buffer is new while a hipGraph is being captured.  Keep gradients persistent "
+                               "(segmi.distributed.DistributedModel does) and run at least one eager step before capturing." % self._name())
+        mats, rest = [], []
+        for gi, g in enumerate(self.param_groups):
+            for p in g["params"]:
+                if p.grad is not None and p.numel():
+                    (mats if self._is_matrix(g, p) else rest).append((gi, p))
+        if mats:
+            k["mats"] = self._matrix_descriptors(mats)
+        if rest:
+            k["rest"] = self._adamw_descriptors(rest)
+            k["rows"] = np.array([self._step_of[p] for _, p in rest])
+        states = [self.state[p] for _, p in mats + rest]
+        held = list(chain.from_iterable(map(dict.values, states)))
+        tensors = flat + [t for st in states for key, t in st.items() if key != "step" and isinstance(t, torch.Tensor)]
+        deep = [i for i, g in enumerate(live) if g.dim() > 1]
+        k.update(flat=flat, missing=missing, grad_ptrs=list(map(_ptr, live)), deep=deep, strides=[live[i].stride() for i in deep], states=states, held=held,
+                 tensors=tensors, ptrs=list(map(_ptr, tensors)), numels=list(map(_numel, flat)), members=mats, shapes=[p.shape for _, p in mats],
+                 lengths=list(map(len, map(_params, self.param_groups))), settings=self._settings())
+        self._kept = k
+        return k
+
+    def _settings(self):
+        return None
+
     def _adamw_descriptors(self, members):
-        """members: [(group index, parameter)] with gradients.  Descriptor array of segmi_adamw_step with this step's numbers."""
-        state = self.state
-        sig = []
+        rows = []
         for gi, p in members:
-            st = state[p]
-            if "exp_avg" in st and "exp_avg_sq" in st:
-                sig.append((p.data_ptr(), p.grad.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), id(st.get("step")), gi))
-            else:
-                sig.append(None)
-        if sig != self._sig.get("adamw"):
-            self._refuse_rebuild_in_capture()
-            rows = []
-            for gi, p in members:
-                g = self._checked(p)
-                rows.append((p.data_ptr(), g.data_ptr(), self._buffer(p, "exp_avg").data_ptr(), self._buffer(p, "exp_avg_sq").data_ptr(),
-                             0, 0.0, p.numel(), gi, 0))
-            self._adopt_steps([p for _, p in members])
-            desc = np.array(rows, dtype=_ADAMW_DTYPE)
-            if self.capturable:
-                desc["step_dev"] = [state[p]["step"].data_ptr() for _, p in members]
-            self._desc["adamw"] = desc
-            self._desc["rows"] = np.array([self._step_of[p] for _, p in members])
-            self._sig["adamw"] = [(p.data_ptr(), p.grad.data_ptr(), state[p]["exp_avg"].data_ptr(), state[p]["exp_avg_sq"].data_ptr(),
-                                   id(state[p]["step"]), gi) for gi, p in members]
-        desc = self._desc["adamw"]
-        if not self.capturable:
-            steps = self._steps.numpy()
-            rows = self._desc["rows"]
-            steps[rows] += 1.0
-            desc["step"] = steps[rows]
+            g = self._checked(p)
+            rows.append((p.data_ptr(), g.data_ptr(), self._buffer(p, "exp_avg").data_ptr(), self._buffer(p, "exp_avg_sq").data_ptr(),
+                         0, 0.0, p.numel(), gi, 0))
+        self._adopt_steps([p for _, p in members])
+        desc = np.array(rows, dtype=_ADAMW_DTYPE)
+        if self.capturable:
+            desc["step_dev"] = [self.state[p]["step"].data_ptr() for _, p in members]
         return desc
 
     def _adopt_steps(self, params):
@@ -242,11 +281,6 @@ class _FusedOptimizer(torch.optim.Optimizer):
         for p, i in self._step_of.items():
             self.state[p]["step"] = self._views[i]
 
-    def _refuse_rebuild_in_capture(self):
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("%s: a parameter, gradient or state buffer is new while a hipGraph is being captured.  Keep gradients persistent "
-                               "(segmi.distributed.DistributedModel does) and run at least one eager step before capturing." % self._name())
-
     def _hyper_values(self):
         raise NotImplementedError
 
@@ -258,7 +292,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("%s.push_hyper must stay outside the captured region (call it before graph replay)" % self._name())
         values = np.concatenate([v.reshape(-1).view(np.uint8) for v in self._hyper_values()])
-        with torch.cuda.device(self._device()):
+        with _on(self._device()):
             if self._hyper is None:
                 self._hyper = _Hyper(values.size, self._device())
             self._hyper.push(values)
@@ -281,15 +315,17 @@ class _FusedOptimizer(torch.optim.Optimizer):
                 h[i, 0] *= float(g[lr_ratio])
         return h
 
-    def _adamw_launch(self, members, hyper, hyper_dev):
-        desc = self._adamw_descriptors(members)
-        ng, n = len(self.param_groups), len(desc)
-        ws = torch.empty(8 * n, dtype=torch.uint8, device=self._device()) if self.capturable else None
-        check(lib.segmi_adamw_step(desc.ctypes.data, n, hyper.ctypes.data, ng, hyper_dev, None if ws is None else ws.data_ptr(),
-                                   0 if ws is None else 8 * n, torch.cuda.current_stream().cuda_stream), "adamw_step")
-
-    def _live(self):
-        return [(gi, p) for gi, g in enumerate(self.param_groups) for p in g["params"] if p.grad is not None and p.numel()]
+    def _adamw_launch(self, k, hyper, hyper_dev, stream):
+        desc, ws, nbytes = k["rest"], None, 0
+        if self.capturable:
+            nbytes = 8 * len(desc)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self._device())
+        else:
+            steps = self._steps.numpy()
+            steps[k["rows"]] += 1.0
+            desc["step"] = steps[k["rows"]]
+        check(lib.segmi_adamw_step(desc.ctypes.data, len(desc), hyper.ctypes.data, len(self.param_groups), hyper_dev,
+                                   None if ws is None else ws.data_ptr(), nbytes, stream), "adamw_step")
 
 
 def _check_common(name, lr, weight_decay, betas, eps):
@@ -321,11 +357,11 @@ class FusedAdamW(_FusedOptimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        members = self._live()
-        if members:
-            with torch.cuda.device(self._device()):
+        k = self._plan()
+        if k["rest"] is not None:
+            with _on(self._device()):
                 self._ready()
-                self._adamw_launch(members, self._hyper_values()[0], self._hyper.dev.data_ptr() if self.capturable else None)
+                self._adamw_launch(k, self._hyper_values()[0], self._hyper.dev.data_ptr() if self.capturable else None, torch.cuda.current_stream().cuda_stream)
         return loss
 
 
@@ -388,28 +424,27 @@ class Muon(_FusedOptimizer):
             h[:, i] = float(g["lr"]), float(g["weight_decay"]), float(g["momentum"])
         return [h, self._adamw_hyper("adamw_betas", "adamw_eps", "adamw_lr_ratio")]
 
-    def _muon_descriptors(self, members):
-        state = self.state
-        sig = [(p.data_ptr(), p.grad.data_ptr(), b.data_ptr() if b is not None else 0, gi, self.param_groups[gi]["adjust_lr_fn"])
-               for gi, p in members for b in (state[p].get("momentum_buffer"),)]
-        if sig != self._sig.get("muon"):
-            self._refuse_rebuild_in_capture()
-            rows = []
-            for gi, p in members:
-                g, (r, c) = self._checked(p), _matrix_of(p)
-                k, rest = p.shape[0], p.numel() // p.shape[0]
-                if self.param_groups[gi]["adjust_lr_fn"] == "match_rms_adamw":
-                    f = 0.2 * math.sqrt(max(k, rest))
-                else:
-                    f = math.sqrt(max(1.0, k / rest))
-                rows.append((p.data_ptr(), g.data_ptr(), self._buffer(p, "momentum_buffer").data_ptr(), r, c, f, gi))
-            desc = self._desc["muon"] = np.array(rows, dtype=_MUON_DTYPE)
-            self._desc["bytes"] = lib.segmi_muon_workspace(desc.ctypes.data, len(desc))
-            if not self._desc["bytes"]:
-                raise SegmiError("segmi.optim.Muon: a matrix is too large (4 GiB of float32 after padding its sides to 64)")
-            self._sig["muon"] = [(p.data_ptr(), p.grad.data_ptr(), state[p]["momentum_buffer"].data_ptr(), gi, self.param_groups[gi]["adjust_lr_fn"])
-                                 for gi, p in members]
-        return self._desc["muon"]
+    def _is_matrix(self, group, p):
+        return group.get("algorithm", "auto") == "auto" and _matrix_of(p) is not None
+
+    def _settings(self):
+        return [(g["adjust_lr_fn"], g.get("algorithm", "auto")) for g in self.param_groups]
+
+    def _matrix_descriptors(self, members):
+        rows = []
+        for gi, p in members:
+            g, (r, c) = self._checked(p), _matrix_of(p)
+            k, rest = p.shape[0], p.numel() // p.shape[0]
+            if self.param_groups[gi]["adjust_lr_fn"] == "match_rms_adamw":
+                f = 0.2 * math.sqrt(max(k, rest))
+            else:
+                f = math.sqrt(max(1.0, k / rest))
+            rows.append((p.data_ptr(), g.data_ptr(), self._buffer(p, "momentum_buffer").data_ptr(), r, c, f, gi))
+        desc = np.array(rows, dtype=_MUON_DTYPE)
+        nbytes = lib.segmi_muon_workspace(desc.ctypes.data, len(desc))
+        if not nbytes:
+            raise SegmiError("segmi.optim.Muon: a matrix is too large (4 GiB of float32 after padding its sides to 64)")
+        return desc, nbytes
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -422,25 +457,21 @@ class Muon(_FusedOptimizer):
         for g in groups[1:]:
             if any(g[k] != first[k] for k in self._SHARED):
                 raise ValueError("segmi.optim.Muon: %s must be the same in all parameter groups" % ", ".join(self._SHARED))
-        mats, rest = [], []
-        for gi, p in self._live():
-            is_matrix = groups[gi].get("algorithm", "auto") == "auto" and _matrix_of(p) is not None
-            (mats if is_matrix else rest).append((gi, p))
-        if not mats and not rest:
+        k = self._plan()
+        if k["mats"] is None and k["rest"] is None:
             return loss
         coef = _check_iteration(first["ns_steps"], first["ns_coefficients"], first["eps"], "segmi.optim.Muon")
-        with torch.cuda.device(self._device()):
+        with _on(self._device()):
             self._ready()
             hd = self._hyper.dev.data_ptr() if self.capturable else None
             h, a = self._hyper_values()
-            ng = len(groups)
-            if mats:
-                desc = self._muon_descriptors(mats)
-                nbytes = self._desc["bytes"]
+            stream = torch.cuda.current_stream().cuda_stream
+            if k["mats"] is not None:
+                desc, nbytes = k["mats"]
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=self._device())
-                check(lib.segmi_muon_step(desc.ctypes.data, len(desc), h[0].ctypes.data, h[1].ctypes.data, h[2].ctypes.data, ng, hd,
+                check(lib.segmi_muon_step(desc.ctypes.data, len(desc), h[0].ctypes.data, h[1].ctypes.data, h[2].ctypes.data, len(groups), hd,
                                           1 if first["nesterov"] else 0, coef, int(first["ns_steps"]), float(first["eps"]), ws.data_ptr(), nbytes,
-                                          torch.cuda.current_stream().cuda_stream), "muon_step")
-            if rest:
-                self._adamw_launch(rest, a, hd + 4 * 3 * _MAX_GROUPS if hd else None)
+                                          stream), "muon_step")
+            if k["rest"] is not None:
+                self._adamw_launch(k, a, hd + 4 * 3 * _MAX_GROUPS if hd else None, stream)
         return loss
