@@ -38,7 +38,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int BATCH = 48;            // matrices per launch: their descriptors travel as kernel arguments (< 4 KiB)
+constexpr int BATCH = 60;            // matrices per launch: their descriptors travel as kernel arguments (< 4 KiB)
 constexpr int MAX_GROUPS = 8;
 constexpr unsigned LINE = 64, LINE_K = 16;   // bytes, values
 
@@ -127,10 +127,11 @@ struct Source {
     long so, si;                     // strides in elements
     int outer, inner;
     unsigned part, parts;            // its partial sums of squares
-    int dtype;                       // 0 fp32, 1 bf16
-    int inner_is_n;                  // 1: the inner dimension is the longer side
-    int group;
+    signed char dtype;               // 0 fp32, 1 bf16
+    signed char inner_is_n;          // 1: the inner dimension is the longer side
+    signed char group;
 };
+static_assert(sizeof(Source) == 64, "sixty of them fit the kernel arguments");
 struct SourceBatch {
     char* ws;
     double* partial;
@@ -725,6 +726,7 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_finish(TargetBatch b, Hyper
 //     X <- a X + Q X    X goes into the instruction as it lies in the registers: the sum over rows may run in any order, so Q's words
 //                       are read in the order in which a lane holds the rows
 // Bound by latency: 64 x 576 is 25 MFLOP a step on one CU (2.7 us at its peak rate) plus four barriers.
+enum Class { SMALL_1_1, SMALL_1_3, SMALL_1_9, SMALL_2_1, SMALL_2_3, SQUARE, WIDE_MATRIX, CLASSES };    // SMALL_R_G
 struct SmallItem {
     const void* src;                 // MUON: the gradient
     void* dst;                       // MUON: the parameter
@@ -732,12 +734,12 @@ struct SmallItem {
     long si, sj, di, dj;             // strides of X's rows and columns in src (and mom), and in dst
     int m, n;
     float factor;
-    int dtype, group;
+    int dtype, group, cls;
     unsigned src_bytes, dst_bytes;   // up to the last element
 };
 struct SmallStep {
     float gram, quad, lin, apply;    // fp32 sums to the next stored scale; X <- a X + Q X keeps X's scale `apply` folded in
-    float alpha;
+    float alpha, ident;
 };
 constexpr int SMALL_BATCH = 32;
 struct SmallBatch {
@@ -833,17 +835,24 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
-template <int R, int G, bool MUON>
-__global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const Hyper* __restrict__ hd) {
-    constexpr int SUBS = R * (R + 1) / 2;                // 32 x 32 subtiles on and below the diagonal
-    constexpr int XP = 36;                               // row pitch in words: ds_read_b128 of 16 rows covers all 64 banks
-    __shared__ __attribute__((aligned(16))) union {
+template <int R>
+struct SmallShared {
+    static constexpr int SUBS = R * (R + 1) / 2;         // 32 x 32 subtiles on and below the diagonal
+    static constexpr int XP = 36;                        // row pitch in words: ds_read_b128 of 16 rows covers all 64 banks
+    union {
         unsigned x[8][32 * R][XP];                       // a wave's slice, turned
         float4 part[8][SUBS][4][64];                     // the waves' sums
     } u;
-    __shared__ __attribute__((aligned(16))) PairPlanes<R> A, Q;
-    __shared__ double red[8];
-    const SmallItem& s = b.item[blockIdx.x];
+    PairPlanes<R> A, Q;
+    double red[8];
+};
+
+template <int R, int G, bool MUON>
+__device__ __forceinline__ void small_matrix(const SmallBatch& b, const SmallItem& s, SmallShared<R>& sh, const Hyper& h, const Hyper* __restrict__ hd) {
+    constexpr int SUBS = SmallShared<R>::SUBS;
+    auto& u = sh.u;
+    PairPlanes<R>&A = sh.A, &Q = sh.Q;
+    double* const red = sh.red;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int m = s.m, n = s.n;
@@ -922,7 +931,10 @@ __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const 
                 w[g][r][p].set(__builtin_amdgcn_ldexpf(x[g][r][2 * p] * factor, power), __builtin_amdgcn_ldexpf(x[g][r][2 * p + 1] * factor, power));
 
     for (int step = 0; step < b.steps; ++step) {
-        const SmallStep k = b.step[step];
+        SmallStep k = b.step[step];
+        // One singular value, 1 from the start, is where a and Q cancel (0.7 = 3.44 - 2.74): there the sum is taken before it is rounded.
+        if (m == 1) k.alpha = 0.f;
+        else k.ident = 0.f;
         {   // A = X X^T
             f32x16 acc[SUBS], mix[SUBS];
 #pragma unroll
@@ -998,7 +1010,7 @@ __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const 
                 float v[4];
                 A.load(row, c, k.lin, v);
 #pragma unroll
-                for (int y = 0; y < 4; ++y) v[y] = fmaf(acc[4 * e + y] + mix[4 * e + y], k.quad, v[y]);
+                for (int y = 0; y < 4; ++y) v[y] = fmaf(acc[4 * e + y] + mix[4 * e + y], k.quad, v[y] + (row + y == c ? k.ident : 0.f));
                 Q.store(row, c, v, ti != tj);
             }
         }
@@ -1069,6 +1081,24 @@ __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const 
     }
 }
 
+// CLS: the class of all matrices of the launch, or CLASSES: mixed, then it lasts as long as the longest of them (a kernel of its
+// own per class needs fewer registers: 64 x 576 45 us instead of 50)
+template <int CLS, bool MUON>
+__global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const Hyper* __restrict__ hd) {
+    constexpr bool SMALL_LDS = CLS == SMALL_1_1 || CLS == SMALL_1_3 || CLS == SMALL_1_9;
+    __shared__ __attribute__((aligned(16))) char smem[SMALL_LDS ? sizeof(SmallShared<1>) : sizeof(SmallShared<2>)];
+    const SmallItem& s = b.item[blockIdx.x];
+    SmallShared<1>& one = *reinterpret_cast<SmallShared<1>*>(smem);
+    SmallShared<2>& two = *reinterpret_cast<SmallShared<2>*>(smem);
+    switch (CLS == CLASSES ? s.cls : CLS) {
+        case SMALL_1_1: small_matrix<1, 1, MUON>(b, s, one, h, hd); break;
+        case SMALL_1_3: small_matrix<1, 3, MUON>(b, s, one, h, hd); break;
+        case SMALL_1_9: small_matrix<1, 9, MUON>(b, s, one, h, hd); break;
+        case SMALL_2_1: small_matrix<2, 1, MUON>(b, s, two, h, hd); break;
+        default: small_matrix<2, 3, MUON>(b, s, two, h, hd); break;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 // Largest value of |f| on [0, s] for the polynomials of the iteration, and the power-of-two scale that keeps such entries below 2^15
 // (fp16 ends at 65504; a matrix's entries are bounded by its spectral norm).
@@ -1121,11 +1151,10 @@ constexpr double SLACK = 1.0 + 1e-5;                     // what rounding may ad
 constexpr double MAX_BOUND = 4096.0;                     // coefficients whose iterates grow beyond this are refused
 
 // Steps between Gram products: one by one for matrices of nearly square shape and for small ones, else 2, 1, 2, 1, ... (see the head
-// of this file; below 65 rows the sums are so short that fp32 rounds hardly at all, and 2 + 1 + 2 came out at up to 2.2 times its distance)
+// of this file)
 int segment_length(bool wide, int index, int left) { return wide && (index & 1) == 0 && left >= 2 ? 2 : 1; }
-enum Class { SMALL_1_1, SMALL_1_3, SMALL_1_9, SMALL_2_1, SMALL_2_3, SQUARE, WIDE_MATRIX, CLASSES };
-bool is_wide(int m, int n) { return m > 64 && n / 2 >= m; }
-// `span`: bytes from the first to behind the last element; ns_small<R, G> addresses with 32 bits
+bool is_wide(int m, int n) { return n / 2 >= m; }
+// `span`: bytes from the first to behind the last element; small_matrix addresses with 32 bits
 Class class_of(int rows, int cols, size_t span) {
     const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
     if (span < ((size_t)1 << 31)) {
@@ -1339,24 +1368,30 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
 
 // `b` carries the callers' pointers; the steps' scales are filled in here
 template <bool MUON>
-int run_small(Class c, SmallBatch& b, int count, const Bounds& f, int steps, const Hyper& h, const Hyper* hd, hipStream_t st) {
+int run_small(SmallBatch& b, int count, const Bounds& f, int steps, const Hyper& h, const Hyper* hd, hipStream_t st) {
     double s = SLACK, sx = Bounds::scale_for(s);
     b.scale = (float)sx;
     b.steps = steps;
     for (int i = 0; i < steps; ++i) {
-        const double sa = Bounds::scale_for(s * s), sq = Bounds::scale_for(f.max_r(s) * SLACK);
+        const double sa = Bounds::scale_for(s * s), sq = Bounds::scale_for(std::fmax(f.max_r(s), f.max_q(s)) * SLACK);
         s = f.max_p(s) * SLACK;
         const double nsx = Bounds::scale_for(s);
-        b.step[i] = SmallStep{(float)(sa / (sx * sx)), (float)(f.c * sq / (sa * sa)), (float)(f.b * sq / sa), (float)(nsx / (sq * sx)), (float)(f.a * nsx / sx)};
+        b.step[i] = SmallStep{(float)(sa / (sx * sx)), (float)(f.c * sq / (sa * sa)), (float)(f.b * sq / sa), (float)(nsx / (sq * sx)), (float)(f.a * nsx / sx), (float)(f.a * sq)};
         sx = nsx;
     }
     b.unscale = (float)(1.0 / sx);
+    int cls = b.item[0].cls;
+    for (int i = 1; i < count; ++i)
+        if (b.item[i].cls != cls) cls = CLASSES;
     const dim3 grid(count), threads(512);
-    if (c == SMALL_1_1) hipLaunchKernelGGL((ns_small<1, 1, MUON>), grid, threads, 0, st, b, h, hd);
-    else if (c == SMALL_1_3) hipLaunchKernelGGL((ns_small<1, 3, MUON>), grid, threads, 0, st, b, h, hd);
-    else if (c == SMALL_1_9) hipLaunchKernelGGL((ns_small<1, 9, MUON>), grid, threads, 0, st, b, h, hd);
-    else if (c == SMALL_2_1) hipLaunchKernelGGL((ns_small<2, 1, MUON>), grid, threads, 0, st, b, h, hd);
-    else hipLaunchKernelGGL((ns_small<2, 3, MUON>), grid, threads, 0, st, b, h, hd);
+    switch (cls) {
+        case SMALL_1_1: hipLaunchKernelGGL((ns_small<SMALL_1_1, MUON>), grid, threads, 0, st, b, h, hd); break;
+        case SMALL_1_3: hipLaunchKernelGGL((ns_small<SMALL_1_3, MUON>), grid, threads, 0, st, b, h, hd); break;
+        case SMALL_1_9: hipLaunchKernelGGL((ns_small<SMALL_1_9, MUON>), grid, threads, 0, st, b, h, hd); break;
+        case SMALL_2_1: hipLaunchKernelGGL((ns_small<SMALL_2_1, MUON>), grid, threads, 0, st, b, h, hd); break;
+        case SMALL_2_3: hipLaunchKernelGGL((ns_small<SMALL_2_3, MUON>), grid, threads, 0, st, b, h, hd); break;
+        default: hipLaunchKernelGGL((ns_small<CLASSES, MUON>), grid, threads, 0, st, b, h, hd); break;
+    }
     return segmi_launch_status();
 }
 
@@ -1371,17 +1406,17 @@ Shape shape_of(int rows, int cols, bool cols_inner) {
 
 Shape shape_of(const segmi_ns_matrix& a) { return shape_of(a.rows, a.cols, a.src_cs == 1 || a.src_rs != 1); }
 
-// The matrices of a call in batches of one class, those with the longest sums first (what is started last should be short):
+// The matrices of a call in batches of one kind (small, square, wide), those with the longest sums first (what is started last should be short):
 // f(class, indices, how many) in order, until it returns something other than SEGMI_OK.  Batches run one after the other and share
 // the workspace.
 template <typename M, typename F>
 int for_batches(const M* mats, int count, F f) {
     const auto side = [&](int i) { return mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols; };
     std::vector<int> order(count);
-    for (int c = 0; c < CLASSES; ++c) {
+    for (int c = SMALL_2_3; c < CLASSES; ++c) {          // SMALL_2_3 stands for all small classes
         int k = 0;
         for (int i = 0; i < count; ++i)
-            if (class_of(mats[i]) == c) order[k++] = i;
+            if (std::max(class_of(mats[i]), SMALL_2_3) == c) order[k++] = i;
         std::stable_sort(order.begin(), order.begin() + k, [&](int a, int b) { return side(a) > side(b); });
         const int most = c < SQUARE ? SMALL_BATCH : BATCH;
         for (int at = 0; at < k; at += most) {
@@ -1440,9 +1475,9 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
                 const segmi_ns_matrix& a = mats_host[index[i]];
                 const bool wide = a.rows <= a.cols;
                 b.item[i] = SmallItem{a.src, a.dst, nullptr, wide ? a.src_rs : a.src_cs, wide ? a.src_cs : a.src_rs, wide ? a.dst_rs : a.dst_cs,
-                                      wide ? a.dst_cs : a.dst_rs, wide ? a.rows : a.cols, wide ? a.cols : a.rows, 0.f, a.dtype, 0, (unsigned)span_of(a), (unsigned)span_of(a)};
+                                      wide ? a.dst_cs : a.dst_rs, wide ? a.rows : a.cols, wide ? a.cols : a.rows, 0.f, a.dtype, 0, class_of(a), (unsigned)span_of(a), (unsigned)span_of(a)};
             }
-            return run_small<false>(cls, b, k, f, steps, Hyper{}, nullptr, (hipStream_t)stream);
+            return run_small<false>(b, k, f, steps, Hyper{}, nullptr, (hipStream_t)stream);
         }
         Shape shapes[BATCH];
         SourceBatch src{};
@@ -1458,7 +1493,7 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
             o.si = cols_inner ? a.src_cs : a.src_rs;
             o.outer = s.outer;
             o.inner = s.inner;
-            o.dtype = a.dtype;
+            o.dtype = (signed char)a.dtype;
             o.inner_is_n = cols_inner == wide;
             Target& t = dst.item[i];
             t.dst = a.dst;
@@ -1510,9 +1545,9 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
                 const bool wide = a.rows <= a.cols;
                 const long si = wide ? a.cols : 1, sj = wide ? 1 : a.cols;
                 b.item[i] = SmallItem{a.grad, a.param, a.momentum, si, sj, si, sj, wide ? a.rows : a.cols, wide ? a.cols : a.rows, a.factor, 0, a.group,
-                                      (unsigned)span_of(a), (unsigned)span_of(a)};
+                                      class_of(a), (unsigned)span_of(a), (unsigned)span_of(a)};
             }
-            return run_small<true>(cls, b, k, f, steps, h, reinterpret_cast<const Hyper*>(hyper_dev), (hipStream_t)stream);
+            return run_small<true>(b, k, f, steps, h, reinterpret_cast<const Hyper*>(hyper_dev), (hipStream_t)stream);
         }
         Shape shapes[BATCH];
         SourceBatch src{};
@@ -1531,7 +1566,7 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
             o.outer = s.outer;
             o.inner = s.inner;
             o.inner_is_n = wide;
-            o.group = a.group;
+            o.group = (signed char)a.group;
             Target& t = dst.item[i];
             t.dst = a.param;
             t.si = wide ? a.cols : 1;
