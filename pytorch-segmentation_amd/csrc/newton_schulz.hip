@@ -294,14 +294,14 @@ __global__ __launch_bounds__(256) void ns_normalise(SourceBatch b, Hyper h, cons
 }
 
 // ------------------------------------------------------------------------------------------------ products
-// One workgroup's BT x BT tile of L R^T over the lines q0 .. q1-1 of both operands: 4 waves in 2 x 2, two workgroups per CU.  A step is
-// U lines, 16 KiB of LDS, four of which are in use: one is multiplied while the copies of the next three are on their way.
+// One workgroup's BT x BT tile of L R^T over the lines q0 .. q1-1 of both operands: 4 waves in 2 x 2.  A step is U lines; one is
+// multiplied while the copies of the next STAGES - 1 are on their way.
 // LDS chunk c (16 B) of a row sits at c ^ ((row >> 2) & 3): 16 consecutive rows, which one ds_read_b128 phase reads, then cover all 64 banks;
 // the permutation is applied to the copy's source address.
-// Per step: the wave waits for ITS copies of the step (those of two later ones may be in flight), the barrier makes all waves' visible
-// and the step before it free, and the copies of the step three ahead go there, one every few products: requested in one go the copies of
+// Per step: the wave waits for ITS copies of the step (those of STAGES - 2 later ones may be in flight), the barrier makes all waves'
+// visible and the step before it free, and the copies of the step STAGES - 1 ahead go there, one every few products: requested in one go the copies of
 // the waves keep each of them from issuing products for the 16 cycles a copy occupies the CU's address path.
-struct Wide { static constexpr int BT = 128, U = 1, PER_CU = 2; static constexpr unsigned STAGES = 4; };
+struct Wide { static constexpr int BT = 128, U = 1, PER_CU = 3; static constexpr unsigned STAGES = 3; };
 struct Many { static constexpr int BT = 64, U = 1, PER_CU = 4; static constexpr unsigned STAGES = 4; };
 struct Few { static constexpr int BT = 64, U = 2, PER_CU = 1; static constexpr unsigned STAGES = 8; };
 
@@ -313,8 +313,8 @@ struct Tile {
     static constexpr unsigned STAGE = 2 * ROWS * U, STAGES = C::STAGES;
     static constexpr int PIECES = BT / 64;               // 1 KiB copies (16 rows) per wave, operand and line
     static constexpr int PER = 2 * PIECES * U;           // copies per wave and step
-    static constexpr int PITCH = BT + 8;                 // see `park`
-    static constexpr unsigned SMEM = STAGES * STAGE > BT * PITCH * 4 ? STAGES * STAGE : BT * PITCH * 4;
+    static constexpr int PITCH = BT + 8;                 // see store_rows
+    static constexpr unsigned SMEM = STAGES * STAGE > 64 * PITCH * 4 ? STAGES * STAGE : 64 * PITCH * 4;
     f32x16 acc[S][S];
 
     // This wave's LDS reads are back and at most N of its copies are in flight; then every wave's are.  The builtin, not asm: the
@@ -367,8 +367,8 @@ struct Tile {
         const int hi = (fk ^ sw) * 16, lo = ((fk + 2) ^ sw) * 16;
         const char* const sl = smem + (wr * S * 32 + fr) * LINE;
         const char* const sr = smem + ROWS + (wc * S * 32 + fr) * LINE;
-        auto step = [&](unsigned k, auto more) {
-            const unsigned at = (k % STAGES) * STAGE;
+        auto step = [&](unsigned k, unsigned stage, unsigned into, auto more) {
+            const unsigned at = stage * STAGE;
             f16x8 lh[U][S], ll[U][S], rh[U][S], rl[U][S];
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -396,15 +396,17 @@ struct Tile {
                             if (t == 2) mix[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[u][i], rl[u][j], mix[i][j], 0, 0, 0);
                             if (decltype(more)::value && (((u * 3 + t) * S + i) * S + j) % EACH == 0 && done < PER) {
                                 __builtin_amdgcn_sched_barrier(0);
-                                copy(k + STAGES - 1, (k + STAGES - 1) % STAGES, done++);
+                                copy(k + STAGES - 1, into, done++);
                                 __builtin_amdgcn_sched_barrier(0);
                             }
                         }
         };
-        unsigned k = 0;
+        unsigned k = 0, stage = 0, before = STAGES - 1;
         for (; k + STAGES - 1 < n; ++k) {
             wait_all<(STAGES - 2) * PER>();
-            step(k, std::true_type{});
+            step(k, stage, before, std::true_type{});
+            before = stage;
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
         for (; k < n; ++k) {                             // everything is under way or here
             switch (n - 1 - k < STAGES - 2 ? n - 1 - k : STAGES - 2) {
@@ -416,7 +418,8 @@ struct Tile {
                 case 5: wait_all<5 * PER>(); break;
                 default: wait_all<6 * PER>(); break;
             }
-            step(k, std::false_type{});
+            step(k, stage, 0, std::false_type{});
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
 #pragma unroll
         for (int i = 0; i < S; ++i)
@@ -426,9 +429,9 @@ struct Tile {
                 for (int x = 0; x < 16; ++x) acc[i][j][x] += mix[i][j][x];
     }
 
-    // f(row, col, v) per 32 x 32 subtile: v[4 g + x] is row `row` + 8 g + x of column `col` (tile-relative)
+    // f(row, col, v) per 32 x 32 subtile: v[4 g + x] is row `row` + 8 g + x of column `col` (tile-relative); what f makes of v stays
     template <typename F>
-    __device__ __forceinline__ void each(F f) const {
+    __device__ __forceinline__ void each(F f) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 #pragma unroll
         for (int i = 0; i < S; ++i)
@@ -438,27 +441,37 @@ struct Tile {
 #pragma unroll
                 for (int x = 0; x < 16; ++x) v[x] = acc[i][j][x];
                 f(((wave >> 1) * S + i) * 32 + 4 * (lane >> 5), ((wave & 1) * S + j) * 32 + (lane & 31), v);
+#pragma unroll
+                for (int x = 0; x < 16; ++x) acc[i][j][x] = v[x];
             }
     }
 
-    // Turning a tile round in LDS: a lane holds runs of rows of one column, a row's line wants runs of columns.  `park` keeps the pair
-    // of a value, `store_rows` writes all parked rows, 16 B a lane.  Pitch: 4 rows apart is 32 banks apart.
-    __device__ __forceinline__ static void park(char* smem, int row, int col, float v) {
-        reinterpret_cast<unsigned*>(smem)[row * PITCH + col] = pair_word(v);
-    }
-    __device__ __forceinline__ static void store_rows(const char* smem, char* out, unsigned lines, unsigned r0, unsigned c0, unsigned rows, unsigned cols) {
-        __syncthreads();
+    // Stores the tile by rows.  A lane holds runs of rows of one column, a row's line wants runs of columns: the tile is turned round in
+    // LDS, 64 rows at a time, as pairs in one word, and written 16 B a lane.  Pitch: 4 rows apart is 32 banks apart.
+    __device__ __forceinline__ void store_rows(char* smem, char* out, unsigned lines, unsigned r0, unsigned c0, unsigned rows, unsigned cols) {
         constexpr int PER_ROW = BT / 8;
-        const int c = (threadIdx.x % PER_ROW) * 8;
-        for (int r = threadIdx.x / PER_ROW; r < BT; r += 256 / PER_ROW) {
-            if (r0 + r >= rows || c0 + c >= cols) continue;
-            const uint4 p = *reinterpret_cast<const uint4*>(smem + (r * PITCH + c) * 4), q = *reinterpret_cast<const uint4*>(smem + (r * PITCH + c) * 4 + 16);
-            uint4 hi, lo;
-            hi.x = (p.x & 0xFFFFu) | p.y << 16; hi.y = (p.z & 0xFFFFu) | p.w << 16; hi.z = (q.x & 0xFFFFu) | q.y << 16; hi.w = (q.z & 0xFFFFu) | q.w << 16;
-            lo.x = p.x >> 16 | (p.y & 0xFFFF0000u); lo.y = p.z >> 16 | (p.w & 0xFFFF0000u); lo.z = q.x >> 16 | (q.y & 0xFFFF0000u); lo.w = q.z >> 16 | (q.w & 0xFFFF0000u);
-            char* const at = out + at_line(lines, r0 + r, c0 + c);
-            *reinterpret_cast<uint4*>(at) = hi;
-            *reinterpret_cast<uint4*>(at + LINE / 2) = lo;
+        unsigned* const words = reinterpret_cast<unsigned*>(smem);
+        const int wave_row = threadIdx.x >> 7, c = (threadIdx.x % PER_ROW) * 8;
+#pragma unroll 1
+        for (int part = 0; part < BT / 64; ++part) {
+            __syncthreads();                             // the stages, or the part before, are done with
+            if (BT == 64 || wave_row == part)
+                each([&](int row, int col, float* v) {
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) words[((row & 63) + 8 * (x >> 2) + (x & 3)) * PITCH + col] = pair_word(v[x]);
+                });
+            __syncthreads();
+            for (int r = threadIdx.x / PER_ROW; r < 64; r += 256 / PER_ROW) {
+                const unsigned row = r0 + 64 * part + r;
+                if (row >= rows || c0 + c >= cols) continue;
+                const uint4 p = *reinterpret_cast<const uint4*>(words + r * PITCH + c), q = *reinterpret_cast<const uint4*>(words + r * PITCH + c + 4);
+                uint4 hi, lo;
+                hi.x = (p.x & 0xFFFFu) | p.y << 16; hi.y = (p.z & 0xFFFFu) | p.w << 16; hi.z = (q.x & 0xFFFFu) | q.y << 16; hi.w = (q.z & 0xFFFFu) | q.w << 16;
+                lo.x = p.x >> 16 | (p.y & 0xFFFF0000u); lo.y = p.z >> 16 | (p.w & 0xFFFF0000u); lo.z = q.x >> 16 | (q.y & 0xFFFF0000u); lo.w = q.z >> 16 | (q.w & 0xFFFF0000u);
+                char* const at = out + at_line(lines, row, c0 + c);
+                *reinterpret_cast<uint4*>(at) = hi;
+                *reinterpret_cast<uint4*>(at + LINE / 2) = lo;
+            }
         }
     }
 };
@@ -501,7 +514,6 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_square_product(Batch b, Pro
     char* const out = base + buffer_offset(pr.out, s.m, s.n);
     const char* const a = base + buffer_offset(A, s.m, s.n);
     const bool mirror = ti != tj;
-    if (mirror) __syncthreads();                         // every wave is done with the stages
     t.each([&](int row, int col, float* v) {
         const unsigned r = ti * BT + row, c = tj * BT + col;
         const bool in = r < M && c < M;                  // (all 32 rows of a subtile or none)
@@ -513,13 +525,12 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_square_product(Batch b, Pro
         for (int x = 0; x < 16; ++x) {
             v[x] *= pr.scale;
             if (POLY) v[x] += pr.lin * av[x] + (r + 8 * (x >> 2) + (x & 3) == c && c < (unsigned)s.m ? pr.ident : 0.f);
-            if (mirror) Tile<C>::park(smem, row + 8 * (x >> 2) + (x & 3), col, v[x]);
         }
         if (in)
 #pragma unroll
             for (int g = 0; g < 4; ++g) store4(out, lines, c, r + 8 * g, v + 4 * g);
     });
-    if (mirror) Tile<C>::store_rows(smem, out, lines, ti * BT, tj * BT, M, M);
+    if (mirror) t.store_rows(smem, out, lines, ti * BT, tj * BT, M, M);
 }
 
 // Gram products A = X X^T: few tiles, long sums.  The sum is cut into `splits` runs of lines, each workgroup leaves its fp32 tile in
@@ -625,7 +636,6 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_apply(Batch b, int p, int t
     char* const xo = base;
     char* const to = base + buffer_offset(tout, s.m, s.n);
     const char* const ti4 = base + buffer_offset(tin, s.m, s.n);
-    __syncthreads();
     t.each([&](int row, int col, float* v) {
         const unsigned r = ti * BT + row, c = tj * BT + col;
         const bool in = r < M && c < N;
@@ -637,13 +647,12 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_apply(Batch b, int p, int t
         for (int x = 0; x < 16; ++x) {
             v[x] *= scale;
             if (alpha != 0.f && in) v[x] = fmaf(alpha, old[x], v[x]);
-            Tile<C>::park(smem, row + 8 * (x >> 2) + (x & 3), col, v[x]);
         }
         if (in)
 #pragma unroll
             for (int g = 0; g < 4; ++g) store4(to, M / LINE_K, c, r + 8 * g, v + 4 * g);
     });
-    Tile<C>::store_rows(smem, xo, N / LINE_K, ti * BT, tj * BT, M, N);
+    t.store_rows(smem, xo, N / LINE_K, ti * BT, tj * BT, M, N);
 }
 
 // the last product goes straight to where the caller wants it
