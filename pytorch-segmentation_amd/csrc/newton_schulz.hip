@@ -155,10 +155,20 @@ __device__ __forceinline__ unsigned short f32_to_bf16(float f) {
 __device__ __forceinline__ float source_at(const Source& s, long off) {
     return s.dtype ? bf16_to_f32(static_cast<const unsigned short*>(s.src)[off]) : static_cast<const float*>(s.src)[off];
 }
+// four neighbours of the inner dimension in one load
+__device__ __forceinline__ bool by_fours(const Source& s) {
+    return s.si == 1 && (s.so & 3) == 0 && (s.inner & 3) == 0 && ((size_t)s.src & (s.dtype ? 7 : 15)) == 0 && ((size_t)s.mom & 15) == 0;
+}
+__device__ __forceinline__ float4 source_four(const Source& s, long off) {
+    if (!s.dtype) return ld4(static_cast<const float*>(s.src) + off);
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(s.src) + off);
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
+}
 
 // Sum of squares of every update in fp64 (a gradient of 1e-25 or 1e25 must not vanish or overflow), one partial per 64 x 256
 // elements, summed later in a fixed order.  MUON also advances the momentum buffer: mom = mu mom + g.
-// HBM-bound: 4 B (MUON 12 B) per element.
+// HBM-bound: 4 B (MUON 12 B) per element.  A wave has four rows under way at a time: one, and bf16 by single elements,
+// took 9.9 instead of 6.6 us for 1024 x 4608 and 37 instead of 14 us for 28 M elements in bf16.
 template <bool MUON>
 __global__ __launch_bounds__(256) void ns_sum_squares(SourceBatch b, Hyper h, const Hyper* __restrict__ hd) {
     const int it = find_item(b, blockIdx.x);
@@ -170,43 +180,54 @@ __global__ __launch_bounds__(256) void ns_sum_squares(SourceBatch b, Hyper h, co
     const float mu = MUON ? (hd ? hd->mom[s.group] : h.mom[s.group]) : 0.f;
     const bool nest = MUON && b.nesterov;
     double sum = 0.0;
-    const bool vec = s.dtype == 0 && s.si == 1 && (s.so & 3) == 0 && (s.inner & 3) == 0 && ((size_t)s.src & 15) == 0 && ((size_t)s.mom & 15) == 0;
-    for (int r = wave; r < 64; r += 4) {
-        const long o = o0 + r;
-        if (o >= s.outer) break;
+    const bool vec = by_fours(s);
+    const auto add = [&](float g, float& m) {            // the update's square; the momentum advanced
+        if (MUON) {
+            m = fmaf(mu, m, g);
+            g = nest ? fmaf(mu, m, g) : m;
+        }
+        sum = fma((double)g, (double)g, sum);
+    };
+#pragma unroll 1
+    for (int r0 = wave; r0 < 64 && o0 + r0 < s.outer; r0 += 16) {
         if (vec) {
             const long i = i0 + lane * 4;
-            if (i < s.inner) {
-                const long off = o * s.so + i;
-                const float4 gv = ld4(static_cast<const float*>(s.src) + off);
-                float g[4] = {gv.x, gv.y, gv.z, gv.w};
-                if (MUON) {
-                    const float4 mv = ld4(s.mom + off);
-                    float m[4] = {mv.x, mv.y, mv.z, mv.w};
+            float4 g[4], m[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        m[x] = fmaf(mu, m[x], g[x]);
-                        g[x] = nest ? fmaf(mu, m[x], g[x]) : m[x];
-                    }
-                    st4(s.mom + off, make_float4(m[0], m[1], m[2], m[3]));
-                }
+            for (int k = 0; k < 4; ++k) {
+                const long o = o0 + r0 + 4 * k;
+                const bool in = o < s.outer && i < s.inner;
+                g[k] = in ? source_four(s, o * s.so + i) : zero4();
+                m[k] = MUON && in ? ld4(s.mom + o * s.so + i) : zero4();
+            }
 #pragma unroll
-                for (int x = 0; x < 4; ++x) sum = fma((double)g[x], (double)g[x], sum);
+            for (int k = 0; k < 4; ++k) {
+                add(g[k].x, m[k].x);
+                add(g[k].y, m[k].y);
+                add(g[k].z, m[k].z);
+                add(g[k].w, m[k].w);
+                const long o = o0 + r0 + 4 * k;
+                if (MUON && o < s.outer && i < s.inner) st4(s.mom + o * s.so + i, m[k]);
             }
         } else {
-            for (int x = 0; x < 4; ++x) {
-                const long i = i0 + x * 64 + lane;
-                if (i < s.inner) {
-                    const long off = o * s.so + i * s.si;
-                    float g = source_at(s, off);
-                    if (MUON) {
-                        const float m = fmaf(mu, s.mom[off], g);
-                        s.mom[off] = m;
-                        g = nest ? fmaf(mu, m, g) : m;
-                    }
-                    sum = fma((double)g, (double)g, sum);
+            float g[4][4], m[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const long o = o0 + r0 + 4 * k, i = i0 + x * 64 + lane;
+                    const bool in = o < s.outer && i < s.inner;
+                    g[k][x] = in ? source_at(s, o * s.so + i * s.si) : 0.f;
+                    m[k][x] = MUON && in ? s.mom[o * s.so + i * s.si] : 0.f;
                 }
-            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    add(g[k][x], m[k][x]);
+                    const long o = o0 + r0 + 4 * k, i = i0 + x * 64 + lane;
+                    if (MUON && o < s.outer && i < s.inner) s.mom[o * s.so + i * s.si] = m[k][x];
+                }
         }
     }
 #pragma unroll
@@ -247,42 +268,46 @@ __global__ __launch_bounds__(256) void ns_normalise(SourceBatch b, Hyper h, cons
     const unsigned lines_inner = pad64(s.inner) / LINE_K, lines_outer = pad64(s.outer) / LINE_K;
     const float mu = MUON ? (hd ? hd->mom[s.group] : h.mom[s.group]) : 0.f;
     const bool nest = MUON && b.nesterov;
-    const bool vec = s.dtype == 0 && s.si == 1 && (s.so & 3) == 0 && (s.inner & 3) == 0 && ((size_t)s.src & 15) == 0 && ((size_t)s.mom & 15) == 0;
-    const int c4 = (tid & 15) * 4;
-    for (int r = tid >> 4; r < 64; r += 16) {
-        const int o = o0 + r, i = i0 + c4;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (o < s.outer) {
-            const long off = (long)o * s.so + (long)i * s.si;
-            if (vec) {
-                if (i < s.inner) {
-                    const float4 mv = MUON ? ld4(s.mom + off) : zero4();
-                    v[0] = mv.x; v[1] = mv.y; v[2] = mv.z; v[3] = mv.w;
-                    if (!MUON || nest) {
-                        const float4 gv = ld4(static_cast<const float*>(s.src) + off);
-                        v[0] = fmaf(mu, v[0], gv.x); v[1] = fmaf(mu, v[1], gv.y); v[2] = fmaf(mu, v[2], gv.z); v[3] = fmaf(mu, v[3], gv.w);
-                    }
-                }
-            } else {
+    const int r0 = tid >> 4, c4 = (tid & 15) * 4, i = i0 + c4;
+    float u[4][4];                                       // all loads first: behind a store they would wait for it
+    if (by_fours(s)) {
+        float4 g[4], m[4];
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    if (i + x < s.inner) {
-                        const long at = off + x * s.si;
-                        if (MUON) {
-                            v[x] = s.mom[at];
-                            if (nest) v[x] = fmaf(mu, v[x], source_at(s, at));
-                        } else {
-                            v[x] = source_at(s, at);
-                        }
-                    }
-            }
+        for (int k = 0; k < 4; ++k) {
+            const int o = o0 + r0 + 16 * k;
+            const bool in = o < s.outer && i < s.inner;
+            const long off = (long)o * s.so + i;
+            g[k] = in && (!MUON || nest) ? source_four(s, off) : zero4();
+            m[k] = in && MUON ? ld4(s.mom + off) : zero4();
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float gv[4] = {g[k].x, g[k].y, g[k].z, g[k].w}, mv[4] = {m[k].x, m[k].y, m[k].z, m[k].w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) u[k][x] = !MUON ? gv[x] : nest ? fmaf(mu, mv[x], gv[x]) : mv[x];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int o = o0 + r0 + 16 * k;
+                const bool in = o < s.outer && i + x < s.inner;
+                const long off = (long)o * s.so + (long)(i + x) * s.si;
+                const float g = in && (!MUON || nest) ? source_at(s, off) : 0.f, m = in && MUON ? s.mom[off] : 0.f;
+                u[k][x] = !MUON ? g : nest ? fmaf(mu, m, g) : m;
+            }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int r = r0 + 16 * k;
+        float v[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            v[x] = (float)((double)v[x] * inv);
+            v[x] = (float)((double)u[k][x] * inv);
             turn[r][c4 + x] = v[x];
         }
-        store4(direct, lines_inner, o, i, v);
+        store4(direct, lines_inner, o0 + r, i, v);
     }
     __syncthreads();
     for (int r = tid >> 4; r < 64; r += 16) {
@@ -1271,7 +1296,7 @@ Plan plan_batch(const Shape* s, int count) {
 
 // runs the whole iteration of up to BATCH matrices; `src` and `dst` carry the callers' pointers, the rest is filled in here
 template <bool MUON>
-int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count, const Bounds& f, int steps, char* ws,
+int run_batch(bool wide, const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count, const Bounds& f, int steps, char* ws,
               const Hyper& h, const Hyper* hd, hipStream_t st) {
     const Plan plan = plan_batch(shapes, count);
     const GramPlan gp = gram_plan(shapes, count);
@@ -1321,7 +1346,6 @@ int run_batch(const Shape* shapes, SourceBatch& src, TargetBatch& dst, int count
     src.scale = (float)sx;
     hipLaunchKernelGGL((ns_normalise<MUON>), dim3(g_norm), dim3(256), 0, st, src, h, hd);
 
-    const bool wide = is_wide(shapes[0].m, shapes[0].n);
     int tin = T0;
     for (int left = steps, seg = 0; left > 0; ++seg) {
         const int len = segment_length(wide, seg, left);
@@ -1415,6 +1439,11 @@ Shape shape_of(int rows, int cols, bool cols_inner) {
 
 Shape shape_of(const segmi_ns_matrix& a) { return shape_of(a.rows, a.cols, a.src_cs == 1 || a.src_rs != 1); }
 
+// Wide matrices next to square ones go step by step with them while a second chain of 22 launches costs more than their two additional products
+// each: 150 x 257 with 512 x 2048 175 instead of 288 us, with 1024 x 2048 263 / 360, with 1024 x 4608 436 / 467, with 4 of 512 x 4608
+// 441 / 455.
+constexpr size_t JOIN_WORK = (size_t)1 << 32;            // sum of m^2 n
+
 // The matrices of a call in batches of one kind (small, square, wide), those with the longest sums first (what is started last should be short):
 // f(class, indices, how many) in order, until it returns something other than SEGMI_OK.  Batches run one after the other and share
 // the workspace.
@@ -1422,10 +1451,19 @@ template <typename M, typename F>
 int for_batches(const M* mats, int count, F f) {
     const auto side = [&](int i) { return mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols; };
     std::vector<int> order(count);
+    size_t square = 0, wide_work = 0;
+    for (int i = 0; i < count; ++i) {
+        const Class c = class_of(mats[i]);
+        square += c == SQUARE;
+        if (c == WIDE_MATRIX) wide_work += (size_t)pad64(side(i)) * pad64(side(i)) * pad64(std::max(mats[i].rows, mats[i].cols));
+    }
+    const bool join = square && wide_work <= JOIN_WORK;
     for (int c = SMALL_2_3; c < CLASSES; ++c) {          // SMALL_2_3 stands for all small classes
         int k = 0;
-        for (int i = 0; i < count; ++i)
-            if (std::max(class_of(mats[i]), SMALL_2_3) == c) order[k++] = i;
+        for (int i = 0; i < count; ++i) {
+            const Class own = std::max(class_of(mats[i]), SMALL_2_3);
+            if ((join && own == WIDE_MATRIX ? SQUARE : own) == c) order[k++] = i;
+        }
         std::stable_sort(order.begin(), order.begin() + k, [&](int a, int b) { return side(a) > side(b); });
         const int most = c < SQUARE ? SMALL_BATCH : BATCH;
         for (int at = 0; at < k; at += most) {
@@ -1513,7 +1551,7 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
             t.dtype = a.dtype;
             t.turned = t.si == 1 && t.sj != 1;
         }
-        return run_batch<false>(shapes, src, dst, k, f, steps, static_cast<char*>(workspace), Hyper{}, nullptr, (hipStream_t)stream);
+        return run_batch<false>(cls == WIDE_MATRIX, shapes, src, dst, k, f, steps, static_cast<char*>(workspace), Hyper{}, nullptr, (hipStream_t)stream);
     });
 }
 
@@ -1586,7 +1624,7 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
             t.group = a.group;
             t.turned = !wide;
         }
-        return run_batch<true>(shapes, src, dst, k, f, steps, static_cast<char*>(workspace), h, reinterpret_cast<const Hyper*>(hyper_dev),
+        return run_batch<true>(cls == WIDE_MATRIX, shapes, src, dst, k, f, steps, static_cast<char*>(workspace), h, reinterpret_cast<const Hyper*>(hyper_dev),
                                (hipStream_t)stream);
     });
 }
