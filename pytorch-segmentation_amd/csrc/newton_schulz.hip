@@ -29,8 +29,9 @@
 #include "lds_dma.h"
 #include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 #include <type_traits>
-#include <vector>
 
 namespace {
 
@@ -1450,7 +1451,8 @@ constexpr size_t JOIN_WORK = (size_t)1 << 32;            // sum of m^2 n
 template <typename M, typename F>
 int for_batches(const M* mats, int count, F f) {
     const auto side = [&](int i) { return mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols; };
-    std::vector<int> order(count);
+    const std::unique_ptr<int[]> order(new (std::nothrow) int[count]);      // (no exception leaves a C entry)
+    if (!order) return SEGMI_ERR_BADARG;
     size_t square = 0, wide_work = 0;
     for (int i = 0; i < count; ++i) {
         const Class c = class_of(mats[i]);
@@ -1464,10 +1466,10 @@ int for_batches(const M* mats, int count, F f) {
             const Class own = std::max(class_of(mats[i]), SMALL_2_3);
             if ((join && own == WIDE_MATRIX ? SQUARE : own) == c) order[k++] = i;
         }
-        std::stable_sort(order.begin(), order.begin() + k, [&](int a, int b) { return side(a) > side(b); });
+        std::sort(order.get(), order.get() + k, [&](int a, int b) { return side(a) != side(b) ? side(a) > side(b) : a < b; });
         const int most = c < SQUARE ? SMALL_BATCH : BATCH;
         for (int at = 0; at < k; at += most) {
-            const int rc = f((Class)c, order.data() + at, k - at < most ? k - at : most);
+            const int rc = f((Class)c, order.get() + at, k - at < most ? k - at : most);
             if (rc != SEGMI_OK) return rc;
         }
     }
@@ -1477,7 +1479,7 @@ int for_batches(const M* mats, int count, F f) {
 template <typename M, typename F>
 size_t workspace_of(const M* mats, int count, F shape) {
     size_t most = 256;                                   // (small matrices need none; 0 means refused)
-    for_batches(mats, count, [&](Class c, const int* index, int k) {
+    const int rc = for_batches(mats, count, [&](Class c, const int* index, int k) {
         if (c < SQUARE) return (int)SEGMI_OK;
         Shape s[BATCH];
         for (int i = 0; i < k; ++i) s[i] = shape(mats[index[i]]);
@@ -1485,7 +1487,7 @@ size_t workspace_of(const M* mats, int count, F shape) {
         if (p.bytes > most) most = p.bytes;
         return (int)SEGMI_OK;
     });
-    return most;
+    return rc == SEGMI_OK ? most : 0;
 }
 
 }  // namespace

@@ -159,7 +159,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
         self.capturable = bool(capturable)
         self._hyper = None
         self._kept = None                            # what the last step saw and the descriptors made from it, see _plan
-        self._steps = self._step_of = None           # one flat tensor of step numbers; state[p]["step"] are views of it
+        self._steps, self._step_of, self._views = None, {}, []      # one flat host tensor of step numbers; state[p]["step"] are views of it
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -170,14 +170,30 @@ class _FusedOptimizer(torch.optim.Optimizer):
     def _name(self):
         return "segmi.optim." + type(self).__name__
 
+    def __getstate__(self):
+        return dict(super().__getstate__(), capturable=self.capturable)
+
+    def __setstate__(self, state):                   # (torch's load_state_dict comes here too, with everything in place)
+        super().__setstate__(state)
+        for name, value in (("capturable", False), ("_hyper", None), ("_kept", None), ("_steps", None), ("_step_of", {}), ("_views", [])):
+            self.__dict__.setdefault(name, value)
+
     def load_state_dict(self, state_dict):
-        """As torch's, but the buffers become this optimizer's own: torch keeps the tensors of the dictionary where type and device fit,
-        and the kernels here would advance those of the optimizer it came from as well."""
+        """As torch's, but the buffers are this optimizer's own: torch keeps the tensors of the dictionary where type and device fit,
+        and the kernels here would advance those of the optimizer it came from as well.  Buffers that were there keep their place
+        and take the values, so a captured step goes on with what was loaded."""
+        before = {p: dict(st) for p, st in self.state.items()}
         super().load_state_dict(state_dict)
-        for st in self.state.values():
-            for key, v in st.items():
-                if isinstance(v, torch.Tensor):
-                    st[key] = v.clone()
+        with torch.no_grad():
+            for p, st in self.state.items():
+                for key, v in st.items():
+                    if not isinstance(v, torch.Tensor):
+                        continue
+                    own = before.get(p, {}).get(key)
+                    if isinstance(own, torch.Tensor) and own.shape == v.shape and own.dtype == v.dtype and (own.device == v.device or key == "step"):
+                        st[key] = own.copy_(v)
+                    else:
+                        st[key] = v.clone()
         self._kept = None
 
     def _buffer(self, p, key):
@@ -219,7 +235,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
         live = [g for g in grads if g is not None] if True in missing else grads
         k = self._kept
         if (k is not None and len(flat) == len(k["flat"]) and all(map(is_, flat, k["flat"])) and missing == k["missing"] and
-                list(map(_ptr, live)) == k["grad_ptrs"] and [live[i].stride() for i in k["deep"]] == k["strides"]):
+                list(map(_ptr, live)) == k["grad_ptrs"] and self._strides(flat, live, k["deep"], k["shallow"]) == k["strides"]):
             held = list(chain.from_iterable(map(dict.values, k["states"])))
             if (len(held) == len(k["held"]) and all(map(is_, held, k["held"])) and list(map(_ptr, k["tensors"])) == k["ptrs"] and
                     list(map(_numel, flat)) == k["numels"] and [p.shape for _, p in k["members"]] == k["shapes"] and
@@ -241,12 +257,14 @@ class _FusedOptimizer(torch.optim.Optimizer):
             k["mats"] = self._matrix_descriptors(mats)
         if rest:
             k["rest"] = self._adamw_descriptors(rest)
-            k["rows"] = np.array([self._step_of[p] for _, p in rest])
+            k["rows"] = None if self.capturable else np.array([self._step_of[p] for _, p in rest])
         states = [self.state[p] for _, p in mats + rest]
         held = list(chain.from_iterable(map(dict.values, states)))
-        tensors = flat + [t for st in states for key, t in st.items() if key != "step" and isinstance(t, torch.Tensor)]
-        deep = [i for i, g in enumerate(live) if g.dim() > 1]
-        k.update(flat=flat, missing=missing, grad_ptrs=list(map(_ptr, live)), deep=deep, strides=[live[i].stride() for i in deep], states=states, held=held,
+        tensors = flat + [t for st in states for key, t in st.items() if (key != "step" or self.capturable) and isinstance(t, torch.Tensor)]
+        deep = [(i, j) for j, i in enumerate(i for i, g in enumerate(grads) if g is not None) if grads[i].dim() > 1]      # (among the parameters, among the gradients)
+        shallow = [j for j, g in enumerate(live) if g.dim() == 1]
+        k.update(flat=flat, missing=missing, grad_ptrs=list(map(_ptr, live)), deep=deep, shallow=shallow,
+                 strides=self._strides(flat, live, deep, shallow), states=states, held=held,
                  tensors=tensors, ptrs=list(map(_ptr, tensors)), numels=list(map(_numel, flat)), members=mats, shapes=[p.shape for _, p in mats],
                  lengths=list(map(len, map(_params, self.param_groups))), settings=self._settings())
         self._kept = k
@@ -254,6 +272,10 @@ class _FusedOptimizer(torch.optim.Optimizer):
 
     def _settings(self):
         return None
+
+    @staticmethod
+    def _strides(flat, live, deep, shallow):
+        return [(flat[i].stride(), live[j].stride()) for i, j in deep] + [live[j].is_contiguous() for j in shallow]
 
     def _adamw_descriptors(self, members):
         rows = []
@@ -268,14 +290,21 @@ class _FusedOptimizer(torch.optim.Optimizer):
         return desc
 
     def _adopt_steps(self, params):
-        """state[p]["step"] as views of one flat float tensor (on the host, or on the device for graphs), keeping the values."""
-        device = self._device() if self.capturable else torch.device("cpu")
-        mine = self._step_of if self._step_of is not None else {}
+        """state[p]["step"] keeps its value and becomes a view of one flat host tensor; for graphs a float on the device, which stays
+        where it is once it is there: captured steps advance it."""
+        value = lambda p: float(self.state[p]["step"]) if self.state[p].get("step") is not None else 0.0
+        if self.capturable:
+            there = lambda t: isinstance(t, torch.Tensor) and t.device == self._device() and t.dtype == torch.float32 and t.numel() == 1
+            fresh = [p for p in params if not there(self.state[p].get("step"))]
+            if fresh:
+                for p, t in zip(fresh, torch.tensor([value(p) for p in fresh], dtype=torch.float32, device=self._device())):
+                    self.state[p]["step"] = t
+            return
+        mine = self._step_of
         if all(p in mine and self.state[p].get("step") is self._views[mine[p]] for p in params):
             return
-        every = list(dict.fromkeys(list(mine) + list(params)))
-        values = [float(self.state[p]["step"]) if self.state[p].get("step") is not None else 0.0 for p in every]
-        self._steps = torch.tensor(values, dtype=torch.float32, device=device)
+        every = list(dict.fromkeys([p for p in mine if self.state.get(p, {}).get("step") is not None] + list(params)))
+        self._steps = torch.tensor([value(p) for p in every], dtype=torch.float32)
         self._step_of = {p: i for i, p in enumerate(every)}
         self._views = [self._steps[i] for i in range(len(every))]
         for p, i in self._step_of.items():

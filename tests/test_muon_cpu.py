@@ -158,3 +158,17 @@ def test_trainer_resolves_the_optimizers_by_name():
     for name in ("Muon", "FusedAdamW"):
         opt = get(optim, "optimizer", {"optimizer": {"type": name, "args": {"lr": 0.01, "weight_decay": 0.0}}}, p)
         assert type(opt).__name__ == name and type(opt).__module__.startswith("segmi")
+
+
+def test_optimizers_copy_and_pickle():
+    import copy
+    import pickle
+    for cls in (optim.Muon, optim.FusedAdamW):
+        p = torch.nn.Parameter(torch.zeros(4, 4))
+        for opt in (copy.deepcopy(cls([p], lr=0.5, capturable=True)), pickle.loads(pickle.dumps(cls([p], lr=0.5, capturable=True)))):
+            assert opt.capturable and opt.param_groups[0]["lr"] == 0.5
+            opt.step()                               # no gradient: nothing happens
+            opt.param_groups[0]["params"][0].grad = torch.ones(4, 4)
+            with pytest.raises((RuntimeError, AssertionError)):
+                opt.step()
+            opt.load_state_dict(opt.state_dict())
