@@ -529,11 +529,9 @@ def _on_wgrad_stream(weight, tensors, fn):
     dev = weight.device
     side = _WGRAD_SIDE["streams"].get(dev.index)
     if side is None:
-        # SEGMI_WGRAD_STREAM_PRIORITY: HIP stream priority of the side stream (lower number = higher priority; the MI355X range is
-        # {0, -1}).  Default -1: measured in one call at cfg2 (profiles/r03_wgrad_stream_priority.txt) 140.1 img/s against 138.4 /
-        # 138.9 at the compute stream's priority — a filter-gradient launch that is dispatched as soon as it is issued overlaps the
-        # HBM-bound BN-backward kernels that follow on the compute stream instead of queueing behind them.
-        side = _WGRAD_SIDE["streams"][dev.index] = torch.cuda.Stream(device=dev, priority=int(os.environ.get("SEGMI_WGRAD_STREAM_PRIORITY", "-1")))
+        # At the default priority like every stream here: queues of different priorities have hung on this hardware, and a raised
+        # one no longer gains anything (PSPNet-R50 8 x 512 x 512: 53.16 ms a step with it, 53.17 without).
+        side = _WGRAD_SIDE["streams"][dev.index] = torch.cuda.Stream(device=dev)
     main = torch.cuda.current_stream(dev)
     side.wait_stream(main)
     with torch.cuda.stream(side):
