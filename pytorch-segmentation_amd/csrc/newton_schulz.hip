@@ -30,6 +30,7 @@
 #include <algorithm>
 #include <cmath>
 #include <memory>
+#include <mutex>
 #include <new>
 #include <type_traits>
 
@@ -169,7 +170,7 @@ __device__ __forceinline__ float4 source_four(const Source& s, long off) {
 // Sum of squares of every update in fp64 (a gradient of 1e-25 or 1e25 must not vanish or overflow), one partial per 64 x 256
 // elements, summed later in a fixed order.  MUON also advances the momentum buffer: mom = mu mom + g.
 // HBM-bound: 4 B (MUON 12 B) per element.  A wave has four rows under way at a time: one, and bf16 by single elements,
-// took 9.9 instead of 6.6 us for 1024 x 4608 and 37 instead of 14 us for 28 M elements in bf16.
+// took 9.9 instead of 6.6 us for 1024 x 4608 and 37 instead of 14 us for 13 M elements in bf16.
 template <bool MUON>
 __global__ __launch_bounds__(256) void ns_sum_squares(SourceBatch b, Hyper h, const Hyper* __restrict__ hd) {
     const int it = find_item(b, blockIdx.x);
@@ -1271,8 +1272,35 @@ GramPlan gram_plan(const Shape* s, int count) {
     GramPlan g;
     g.config = work128 / 16.0 >= 512.0 ? WIDE : work64 / 16.0 > SEGMI_NUM_CU ? MANY : FEW;
     g.bt = tile_of(g.config);
-    const double run = std::ceil((g.config == WIDE ? work128 / 512.0 : work64 / 1024.0) / 4.0) * 4.0;
-    g.run = run < 16.0 ? 16u : (unsigned)run;            // whole steps of a tile
+    if (g.config != WIDE) {
+        const double run = std::ceil(work64 / 1024.0 / 4.0) * 4.0;
+        g.run = run < 16.0 ? 16u : (unsigned)run;        // whole steps of a tile
+        return g;
+    }
+    // All workgroups are on the card at once, so the CU with one more of them than the others decides: the shortest run that leaves at most
+    // two a CU, or three where that is less work for the fullest one.  (Runs of a 512th of all lines: 2048 x 36864 in 544 workgroups 552 us, in
+    // 680 477; fifty filters of a network 123 -> 108 us.)
+    unsigned longest = 16;
+    for (int i = 0; i < count; ++i) longest = std::max(longest, pad64(s[i].n) / LINE_K);
+    const auto groups = [&](unsigned run) {
+        size_t w = 0;
+        for (int i = 0; i < count; ++i) w += (size_t)low_tiles(s[i].m, 128) * segmi_cdiv(pad64(s[i].n) / LINE_K, run);
+        return w;
+    };
+    double best = 0.0;
+    for (unsigned per = 2; per <= 3; ++per) {
+        unsigned lo = 4, hi = longest / 4;               // the shortest run in units of four lines, if any
+        while (lo < hi) {
+            const unsigned mid = (lo + hi) / 2;
+            if (groups(4 * mid) <= (size_t)per * SEGMI_NUM_CU) hi = mid;
+            else lo = mid + 1;
+        }
+        const double cost = 4.0 * lo * (double)segmi_cdiv((long)groups(4 * lo), SEGMI_NUM_CU);
+        if (best == 0.0 || cost < best) {
+            best = cost;
+            g.run = 4 * lo;
+        }
+    }
     return g;
 }
 
@@ -1429,6 +1457,58 @@ int run_small(SmallBatch& b, int count, const Bounds& f, int steps, const Hyper&
     return segmi_launch_status();
 }
 
+// Small matrices take one CU each for as long as a third of a network's whole step, so next to others they run on a stream of
+// their own, which waits for the caller's and is waited for by it (a whole Muon step of PSPNet's filters 1777 -> 1728 us, of UNet's 1194 -> 1130;
+// five small ones beside 150 x 257 and 333 x 65 242 -> 210 us for a call alone.  The two waits cost the host 25 us.)
+// Inside a capture everything stays on the captured stream: this one may be at work for another thread.
+class Aside {
+    static constexpr int DEVICES = 64;
+    struct Side {
+        hipStream_t stream = nullptr;
+        hipEvent_t event = nullptr;      // recorded and waited for under the lock: a wait keeps the record it saw
+    };
+    static std::mutex& lock() { static std::mutex m; return m; }
+    static Side* sides() { static Side s[DEVICES]; return s; }
+    hipStream_t caller;
+    Side* side = nullptr;
+
+    static bool pass(hipStream_t from, hipEvent_t event, hipStream_t to) {
+        return hipEventRecord(event, from) == hipSuccess && hipStreamWaitEvent(to, event, 0) == hipSuccess;
+    }
+
+public:
+    Aside(hipStream_t st, bool wanted) : caller(st) {
+        int dev = -1;
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (!wanted) return;
+        if (hipStreamIsCapturing(st, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone || hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= DEVICES) {
+            (void)hipGetLastError();
+            return;
+        }
+        const std::lock_guard<std::mutex> hold(lock());
+        Side& s = sides()[dev];
+        if (!s.event && hipEventCreateWithFlags(&s.event, hipEventDisableTiming) != hipSuccess) s.event = nullptr;
+        if (s.event && !s.stream && hipStreamCreateWithFlags(&s.stream, hipStreamNonBlocking) != hipSuccess) s.stream = nullptr;
+        if (s.stream && pass(st, s.event, s.stream)) side = &s;
+        else (void)hipGetLastError();                    // then everything runs on the caller's
+    }
+    hipStream_t stream() const { return side ? side->stream : caller; }
+    // the caller's stream goes on behind both
+    int join(int rc) {
+        if (!side) return rc;
+        const std::lock_guard<std::mutex> hold(lock());
+        const bool ok = pass(side->stream, side->event, caller);
+        return rc != SEGMI_OK ? rc : ok ? SEGMI_OK : SEGMI_ERR_LAUNCH;
+    }
+};
+
+template <typename M>
+bool mixed(const M* mats, int count) {
+    int small = 0;
+    for (int i = 0; i < count; ++i) small += class_of(mats[i]) < SQUARE;
+    return small && small < count;
+}
+
 bool shape_ok(int rows, int cols) {
     return rows > 0 && cols > 0 && big_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows) < ((size_t)1 << 32);
 }
@@ -1516,7 +1596,8 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
     if ((size_t)workspace & 255) return SEGMI_ERR_ALIGN;
     if (workspace_bytes < segmi_ns_workspace(mats_host, count)) return SEGMI_ERR_WORKSPACE;
     const Bounds f{coefficients_host[0], coefficients_host[1], coefficients_host[2]};
-    return for_batches(mats_host, count, [&](Class cls, const int* index, int k) {
+    Aside aside((hipStream_t)stream, mixed(mats_host, count));
+    return aside.join(for_batches(mats_host, count, [&](Class cls, const int* index, int k) {
         if (cls < SQUARE) {
             SmallBatch b{};
             b.eps = eps;
@@ -1526,7 +1607,7 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
                 b.item[i] = SmallItem{a.src, a.dst, nullptr, wide ? a.src_rs : a.src_cs, wide ? a.src_cs : a.src_rs, wide ? a.dst_rs : a.dst_cs,
                                       wide ? a.dst_cs : a.dst_rs, wide ? a.rows : a.cols, wide ? a.cols : a.rows, 0.f, a.dtype, 0, class_of(a), (unsigned)span_of(a), (unsigned)span_of(a)};
             }
-            return run_small<false>(b, k, f, steps, Hyper{}, nullptr, (hipStream_t)stream);
+            return run_small<false>(b, k, f, steps, Hyper{}, nullptr, aside.stream());
         }
         Shape shapes[BATCH];
         SourceBatch src{};
@@ -1554,7 +1635,7 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
             t.turned = t.si == 1 && t.sj != 1;
         }
         return run_batch<false>(cls == WIDE_MATRIX, shapes, src, dst, k, f, steps, static_cast<char*>(workspace), Hyper{}, nullptr, (hipStream_t)stream);
-    });
+    }));
 }
 
 size_t segmi_muon_workspace(const segmi_muon_matrix* mats_host, int count) {
@@ -1584,7 +1665,8 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
             h.wd[i] = weight_decay_host[i];
             h.mom[i] = momentum_host[i];
         }
-    return for_batches(mats_host, count, [&](Class cls, const int* index, int k) {
+    Aside aside((hipStream_t)stream, mixed(mats_host, count));
+    return aside.join(for_batches(mats_host, count, [&](Class cls, const int* index, int k) {
         if (cls < SQUARE) {
             SmallBatch b{};
             b.eps = eps;
@@ -1596,7 +1678,7 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
                 b.item[i] = SmallItem{a.grad, a.param, a.momentum, si, sj, si, sj, wide ? a.rows : a.cols, wide ? a.cols : a.rows, a.factor, 0, a.group,
                                       class_of(a), (unsigned)span_of(a), (unsigned)span_of(a)};
             }
-            return run_small<true>(b, k, f, steps, h, reinterpret_cast<const Hyper*>(hyper_dev), (hipStream_t)stream);
+            return run_small<true>(b, k, f, steps, h, reinterpret_cast<const Hyper*>(hyper_dev), aside.stream());
         }
         Shape shapes[BATCH];
         SourceBatch src{};
@@ -1628,7 +1710,7 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
         }
         return run_batch<true>(cls == WIDE_MATRIX, shapes, src, dst, k, f, steps, static_cast<char*>(workspace), h, reinterpret_cast<const Hyper*>(hyper_dev),
                                (hipStream_t)stream);
-    });
+    }));
 }
 
 }  // extern "C"

@@ -24,6 +24,7 @@ NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 _NS_DTYPE = np.dtype([("src", "<u8"), ("dst", "<u8"), ("src_rs", "<i8"), ("src_cs", "<i8"), ("dst_rs", "<i8"), ("dst_cs", "<i8"),
                       ("rows", "<i4"), ("cols", "<i4"), ("dtype", "<i4"), ("reserved", "<i4")])
+_NS_CODES = {torch.float32: 0, torch.bfloat16: 1}
 _MUON_DTYPE = np.dtype([("param", "<u8"), ("grad", "<u8"), ("momentum", "<u8"), ("rows", "<i4"), ("cols", "<i4"), ("factor", "<f4"), ("group", "<i4")])
 _ADAMW_DTYPE = np.dtype([("param", "<u8"), ("grad", "<u8"), ("exp_avg", "<u8"), ("exp_avg_sq", "<u8"), ("step_dev", "<u8"), ("step", "<f8"),
                          ("count", "<i8"), ("group", "<i4"), ("reserved", "<i4")])
@@ -59,8 +60,8 @@ def _unit_of(sizes, strides):
 
 
 def _matrix_strides(t):
-    """(row stride, column stride) of t seen as shape[0] x rest, columns in the order of memory; None if it has none."""
-    cs = t.stride(1) if t.dim() == 2 else _unit_of(t.shape[1:], t.stride()[1:])
+    """(row stride, column stride) of t, of three or more dimensions, seen as shape[0] x rest, columns in the order of memory; None if it has none."""
+    cs = _unit_of(t.shape[1:], t.stride()[1:])
     return None if cs is None else (t.stride(0), cs)
 
 
@@ -78,7 +79,7 @@ def orthogonalize(matrices, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
     coef = _check_iteration(steps, coefficients, eps, "segmi.optim.orthogonalize")
     outs, rows = [], []
     keep = []                                     # copies of inputs without a matrix order live until the launches are queued
-    device = None
+    device, index = None, -1
     for t in mats:
         if not isinstance(t, torch.Tensor) or t.dim() < 2:
             raise ValueError("segmi.optim.orthogonalize: a tensor of two or more dimensions is needed, got %s" %
@@ -86,25 +87,29 @@ def orthogonalize(matrices, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
         if not t.is_cuda:
             raise SegmiError("segmi.optim.orthogonalize: tensor is on %s — the kernels only run on the MI355X (there is deliberately no "
                              "CPU / eager fallback)" % t.device)
-        if t.dtype not in (torch.float32, torch.bfloat16):
+        code = _NS_CODES.get(t.dtype)
+        if code is None:
             raise SegmiError("segmi.optim.orthogonalize: expected float32 or bfloat16, got %s" % t.dtype)
         if device is None:
-            device = t.device
-        elif t.device != device:
+            device, index = t.device, t.get_device()
+        elif t.get_device() != index:
             raise SegmiError("segmi.optim.orthogonalize: all matrices must be on one device, got %s and %s" % (device, t.device))
         out = torch.empty_like(t)
-        outs.append(out)
-        if t.numel() == 0:
-            continue
-        st = _matrix_strides(t)
-        if st is None or (t.dim() > 2 and out.stride() != t.stride()):
-            t = t.contiguous()
-            keep.append(t)
-            out = outs[-1] = torch.empty_like(t)
+        n = t.numel()
+        if n and t.dim() == 2:
+            st, so = t.stride(), out.stride()
+        elif n:
             st = _matrix_strides(t)
-        so = _matrix_strides(out)
-        r = t.shape[0]
-        rows.append((t.data_ptr(), out.data_ptr(), st[0], st[1], so[0], so[1], r, t.numel() // r, 0 if t.dtype == torch.float32 else 1, 0))
+            if st is None or out.stride() != t.stride():
+                t = t.contiguous()
+                keep.append(t)
+                out = torch.empty_like(t)
+                st = _matrix_strides(t)
+            so = _matrix_strides(out)
+        outs.append(out)
+        if n:
+            r = t.shape[0]
+            rows.append((t.data_ptr(), out.data_ptr(), *st, *so, r, n // r, code, 0))
     if rows:
         desc = np.array(rows, dtype=_NS_DTYPE)
         with torch.cuda.device(device):

@@ -628,3 +628,25 @@ def test_train_main_with_the_optimizer_from_config(cuda, tmp_path, name):
     assert again.start_epoch == 2 and all(torch.isfinite(v) for v in again.iteration_losses)
     steps = {float(st["step"]) for st in again.optimizer.state.values() if "step" in st}
     assert steps == {2.0 * len(tr.iteration_losses)}
+
+
+def test_small_matrices_beside_large_ones_keep_the_callers_order(cuda):
+    """Small matrices run on a stream of their own next to large ones: what the caller queued before a call, and what is queued behind it,
+    stay before and behind, on the default stream and on another, eager and captured."""
+    gen = gen_of(cuda, 31)
+    small, large = matrix("gauss", 30, 200, gen, cuda), matrix("gauss", 200, 900, gen, cuda)
+    busy = torch.zeros(1 << 26, device=cuda)
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            stream.wait_stream(torch.cuda.default_stream())
+            for k in range(4):
+                busy.add_(1.0)                           # keeps the stream occupied while the host goes on
+                a, b = small * (k + 1.0), large + 0.01 * k
+                x, y = optim.orthogonalize([a, b])
+                sums = x.sum() + y.sum()                 # reads what has to be there
+                a.zero_()                                # and overwrites what was read
+                b.zero_()
+                want = optim.orthogonalize([small * (k + 1.0)])[0], optim.orthogonalize([large + 0.01 * k])[0]
+                assert torch.equal(x, want[0]) and torch.equal(y, want[1]), k
+                assert torch.equal(sums, want[0].sum() + want[1].sum())
+        torch.cuda.synchronize()
