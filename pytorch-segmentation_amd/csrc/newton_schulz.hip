@@ -340,8 +340,9 @@ struct Tile {
     static constexpr unsigned STAGE = 2 * ROWS * U, STAGES = C::STAGES;
     static constexpr int PIECES = BT / 64;               // 1 KiB copies (16 rows) per wave, operand and line
     static constexpr int PER = 2 * PIECES * U;           // copies per wave and step
-    static constexpr int PITCH = BT + 8;                 // see store_rows
-    static constexpr unsigned SMEM = STAGES * STAGE > 64 * PITCH * 4 ? STAGES * STAGE : 64 * PITCH * 4;
+    static constexpr int PITCH = S * 32 + 8;             // see store_rows
+    static constexpr unsigned SMEM = STAGES * STAGE;
+    static_assert(SMEM >= 4 * 32 * PITCH * 4, "four waves turn 32 rows each");
     f32x16 acc[S][S];
 
     // This wave's LDS reads are back and at most N of its copies are in flight; then every wave's are.  The builtin, not asm: the
@@ -473,32 +474,33 @@ struct Tile {
             }
     }
 
-    // Stores the tile by rows.  A lane holds runs of rows of one column, a row's line wants runs of columns: the tile is turned round in
-    // LDS, 64 rows at a time, as pairs in one word, and written 16 B a lane.  Pitch: 4 rows apart is 32 banks apart.
+    // Stores the tile by rows.  A lane holds runs of rows of one column, a row's line wants runs of columns: each wave turns its own part
+    // round in LDS, 32 rows at a time, as pairs in one word, and writes them 16 B a lane.  Pitch: 4 rows apart is 32 banks apart.
     __device__ __forceinline__ void store_rows(char* smem, char* out, unsigned lines, unsigned r0, unsigned c0, unsigned rows, unsigned cols) {
-        constexpr int PER_ROW = BT / 8;
-        unsigned* const words = reinterpret_cast<unsigned*>(smem);
-        const int wave_row = threadIdx.x >> 7, c = (threadIdx.x % PER_ROW) * 8;
-#pragma unroll 1
-        for (int part = 0; part < BT / 64; ++part) {
-            __syncthreads();                             // the stages, or the part before, are done with
-            if (BT == 64 || wave_row == part)
-                each([&](int row, int col, float* v) {
+        constexpr int PER_ROW = S * 4;                   // lanes
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (lane % PER_ROW) * 8;
+        unsigned* const words = reinterpret_cast<unsigned*>(smem) + wave * 32 * PITCH;
+        __syncthreads();                                 // the stages are done with
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) words[((row & 63) + 8 * (x >> 2) + (x & 3)) * PITCH + col] = pair_word(v[x]);
-                });
-            __syncthreads();
-            for (int r = threadIdx.x / PER_ROW; r < 64; r += 256 / PER_ROW) {
-                const unsigned row = r0 + 64 * part + r;
-                if (row >= rows || c0 + c >= cols) continue;
+        for (int i = 0; i < S; ++i) {
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) words[(4 * (lane >> 5) + 8 * (x >> 2) + (x & 3)) * PITCH + j * 32 + (lane & 31)] = pair_word(acc[i][j][x]);
+            __builtin_amdgcn_wave_barrier();             // (a wave's LDS operations run in their order)
+#pragma unroll
+            for (int r = lane / PER_ROW; r < 32; r += 64 / PER_ROW) {
+                const unsigned row = r0 + ((wave >> 1) * S + i) * 32 + r, col = c0 + (wave & 1) * S * 32 + c;
                 const uint4 p = *reinterpret_cast<const uint4*>(words + r * PITCH + c), q = *reinterpret_cast<const uint4*>(words + r * PITCH + c + 4);
+                if (row >= rows || col >= cols) continue;
                 uint4 hi, lo;
                 hi.x = (p.x & 0xFFFFu) | p.y << 16; hi.y = (p.z & 0xFFFFu) | p.w << 16; hi.z = (q.x & 0xFFFFu) | q.y << 16; hi.w = (q.z & 0xFFFFu) | q.w << 16;
                 lo.x = p.x >> 16 | (p.y & 0xFFFF0000u); lo.y = p.z >> 16 | (p.w & 0xFFFF0000u); lo.z = q.x >> 16 | (q.y & 0xFFFF0000u); lo.w = q.z >> 16 | (q.w & 0xFFFF0000u);
-                char* const at = out + at_line(lines, row, c0 + c);
+                char* const at = out + at_line(lines, row, col);
                 *reinterpret_cast<uint4*>(at) = hi;
                 *reinterpret_cast<uint4*>(at + LINE / 2) = lo;
             }
+            __builtin_amdgcn_wave_barrier();
         }
     }
 };
