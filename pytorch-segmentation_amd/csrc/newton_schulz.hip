@@ -731,26 +731,35 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_finish(TargetBatch b, Hyper
     t.each([&](int row, int col, float* v) {
         const unsigned c = c0 + col, r = r0 + row;
         if (c >= cols || r >= rows) return;              // (r is the lane's first row)
-        float old4[16], before[16];
-        if (b.alpha != 0.f)
+        if (b.alpha != 0.f) {
+            float old4[16];
 #pragma unroll
             for (int g = 0; g < 4; ++g) load4(old, old_lines, c, r + 8 * g, old4 + 4 * g);    // padded rows: in the buffer
-        if (MUON)                                        // all loads first: behind a store they would wait for it
 #pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const unsigned rr = r + 8 * (x >> 2) + (x & 3);
-                if (rr < rows) before[x] = static_cast<const float*>(s.dst)[(long)rr * sr + (long)c * sc];
+            for (int x = 0; x < 16; ++x) v[x] = fmaf(b.alpha, old4[x], v[x] * b.scale);
+        } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) v[x] *= b.scale;
+        }
+        const long at = (long)r * sr + (long)c * sc;     // and uniform distances from there
+        const auto rows_of = [&](auto* const dst, auto make) {
+            if ((r & ~31u) + 32 <= rows) {               // all of a subtile's rows, for the wave
+#pragma unroll
+                for (int x = 0; x < 16; ++x) make(dst + (8 * (x >> 2) + (x & 3)) * sr, x);
+            } else {
+#pragma unroll
+                for (int x = 0; x < 16; ++x)
+                    if (r + 8 * (x >> 2) + (x & 3) < rows) make(dst + (8 * (x >> 2) + (x & 3)) * sr, x);
             }
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-            const unsigned rr = r + 8 * (x >> 2) + (x & 3);
-            if (rr >= rows) continue;
-            float o = v[x] * b.scale;
-            if (b.alpha != 0.f) o = fmaf(b.alpha, old4[x], o);
-            const long at = (long)rr * sr + (long)c * sc;
-            if (MUON) static_cast<float*>(s.dst)[at] = fmaf(-step, o, before[x] * keep);
-            else if (s.dtype) static_cast<unsigned short*>(s.dst)[at] = f32_to_bf16(o);
-            else static_cast<float*>(s.dst)[at] = o;
+        };
+        if (MUON) {
+            float before[16];                            // all loads first: behind a store they would wait for it
+            rows_of(static_cast<float*>(s.dst) + at, [&](float* p, int x) { before[x] = *p; });
+            rows_of(static_cast<float*>(s.dst) + at, [&](float* p, int x) { *p = fmaf(-step, v[x], before[x] * keep); });
+        } else if (s.dtype) {
+            rows_of(static_cast<unsigned short*>(s.dst) + at, [&](unsigned short* p, int x) { *p = f32_to_bf16(v[x]); });
+        } else {
+            rows_of(static_cast<float*>(s.dst) + at, [&](float* p, int x) { *p = v[x]; });
         }
     });
 }
