@@ -39,6 +39,7 @@ namespace {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int BATCH = 60;            // matrices per launch: their descriptors travel as kernel arguments (< 4 KiB)
 constexpr int MAX_GROUPS = 8;
@@ -112,13 +113,6 @@ __device__ __forceinline__ void store1(char* buf, unsigned lines, unsigned row, 
     *reinterpret_cast<_Float16*>(p) = h;
     *reinterpret_cast<_Float16*>(p + LINE / 2) = l;
 }
-__device__ __forceinline__ void load4(const char* buf, unsigned lines, unsigned row, unsigned k, float* v) {
-    const char* p = buf + at_line(lines, row, k);
-    const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + LINE / 2);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) v[x] = join(hi[x], lo[x]);
-}
-
 // ------------------------------------------------------------------------------------------------ reading the updates
 // An update is seen as outer x inner with the inner dimension the contiguous one where there is one.
 struct Source {
@@ -457,7 +451,8 @@ struct Tile {
                 for (int x = 0; x < 16; ++x) acc[i][j][x] += mix[i][j][x];
     }
 
-    // f(row, col, v) per 32 x 32 subtile: v[4 g + x] is row `row` + 8 g + x of column `col` (tile-relative); what f makes of v stays
+    // f(row, col, v, at) per 32 x 32 subtile: v[4 g + x] is row `row` + 8 g + x of column `col` (tile-relative); what f makes of v
+    // stays; at: see Columns
     template <typename F>
     __device__ __forceinline__ void each(F f) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -468,14 +463,14 @@ struct Tile {
                 float v[16];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) v[x] = acc[i][j][x];
-                f(((wave >> 1) * S + i) * 32 + 4 * (lane >> 5), ((wave & 1) * S + j) * 32 + (lane & 31), v);
+                f(((wave >> 1) * S + i) * 32 + 4 * (lane >> 5), ((wave & 1) * S + j) * 32 + (lane & 31), v, i * 2 * 64 * LINE + j * 32 * LINE);
 #pragma unroll
                 for (int x = 0; x < 16; ++x) acc[i][j][x] = v[x];
             }
     }
 
-    // Stores the tile by rows.  A lane holds runs of rows of one column, a row's line wants runs of columns: each wave turns its own part
-    // round in LDS, 32 rows at a time, as pairs in one word, and writes them 16 B a lane.  Pitch: 4 rows apart is 32 banks apart.
+    // Stores the tile, pairs in one word, by rows.  A lane holds runs of rows of one column, a row's line wants runs of columns: each wave turns its own part
+    // round in LDS, 32 rows at a time, and writes them 16 B a lane.  Pitch: 4 rows apart is 32 banks apart.
     __device__ __forceinline__ void store_rows(char* smem, char* out, unsigned lines, unsigned r0, unsigned c0, unsigned rows, unsigned cols) {
         constexpr int PER_ROW = S * 4;                   // lanes
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (lane % PER_ROW) * 8;
@@ -486,7 +481,7 @@ struct Tile {
 #pragma unroll
             for (int j = 0; j < S; ++j)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) words[(4 * (lane >> 5) + 8 * (x >> 2) + (x & 3)) * PITCH + j * 32 + (lane & 31)] = pair_word(acc[i][j][x]);
+                for (int x = 0; x < 16; ++x) words[(4 * (lane >> 5) + 8 * (x >> 2) + (x & 3)) * PITCH + j * 32 + (lane & 31)] = __float_as_uint(acc[i][j][x]);
             __builtin_amdgcn_wave_barrier();             // (a wave's LDS operations run in their order)
 #pragma unroll
             for (int r = lane / PER_ROW; r < 32; r += 64 / PER_ROW) {
@@ -502,6 +497,41 @@ struct Tile {
             }
             __builtin_amdgcn_wave_barrier();
         }
+    }
+};
+
+// A matrix whose rows are a tile's columns (the transpose, or a symmetric one).  A lane's place in it is computed once; the subtiles and register
+// groups lie at distances that are the same for all lanes.  Loads from beyond the buffer give zeros; what lies beyond the last row is not stored.
+struct Columns {
+    i32x4 rsrc;
+    unsigned at;
+    template <typename C>
+    static __device__ __forceinline__ Columns of(const Tile<C>&, const char* buf, unsigned rows, unsigned lines, unsigned r0, unsigned c0) {
+        constexpr int S = Tile<C>::S;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        return Columns{make_rsrc(buf, rows * lines * LINE),
+                       (unsigned)at_line(lines, c0 + (wave & 1) * S * 32 + (lane & 31), r0 + (wave >> 1) * S * 32 + 4 * (lane >> 5))};
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer() const {
+        return __builtin_amdgcn_make_buffer_rsrc((void*)((unsigned long long)(unsigned)rsrc.x | (unsigned long long)(unsigned)rsrc.y << 32), 0, rsrc.z, rsrc.w);
+    }
+    // rows 8 g .. 8 g + 3 of a subtile, as pairs in one word
+    __device__ __forceinline__ void store(unsigned sub, int g, const float* v) const {
+        unsigned w[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) w[x] = __float_as_uint(v[x]);
+        const u32x2 hi = {(w[0] & 0xFFFFu) | w[1] << 16, (w[2] & 0xFFFFu) | w[3] << 16};
+        const u32x2 lo = {w[0] >> 16 | (w[1] & 0xFFFF0000u), w[2] >> 16 | (w[3] & 0xFFFF0000u)};
+        const unsigned to = at + (g & 1) * 16, up = sub + (g >> 1) * 64 * LINE;
+        __builtin_amdgcn_raw_buffer_store_b64(hi, buffer(), to, up, 0);
+        __builtin_amdgcn_raw_buffer_store_b64(lo, buffer(), to + LINE / 2, up, 0);
+    }
+    __device__ __forceinline__ void load(unsigned sub, int g, float* v) const {
+        const unsigned from = at + (g & 1) * 16, up = sub + (g >> 1) * 64 * LINE;
+        const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_raw_buffer_load_b64(buffer(), from, up, 0));
+        const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_raw_buffer_load_b64(buffer(), from + LINE / 2, up, 0));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = join(hi[x], lo[x]);
     }
 };
 
@@ -541,23 +571,23 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_square_product(Batch b, Pro
     Tile<C> t;
     t.run(smem, base + buffer_offset(pr.l, s.m, s.n), M, base + buffer_offset(pr.r, s.m, s.n), M, lines, ti * BT, tj * BT, 0, lines);
     char* const out = base + buffer_offset(pr.out, s.m, s.n);
-    const char* const a = base + buffer_offset(A, s.m, s.n);
+    const Columns a = Columns::of(t, base + buffer_offset(A, s.m, s.n), M, lines, ti * BT, tj * BT), o = Columns::of(t, out, M, lines, ti * BT, tj * BT);
     const bool mirror = ti != tj;
-    t.each([&](int row, int col, float* v) {
+    t.each([&](int row, int col, float* v, unsigned at) {
         const unsigned r = ti * BT + row, c = tj * BT + col;
-        const bool in = r < M && c < M;                  // (all 32 rows of a subtile or none)
         float av[16];
-        if (POLY && in)
+        if (POLY)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) load4(a, lines, c, r + 8 * g, av + 4 * g);
+            for (int g = 0; g < 4; ++g) a.load(at, g, av + 4 * g);
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
             v[x] *= pr.scale;
             if (POLY) v[x] += pr.lin * av[x] + (r + 8 * (x >> 2) + (x & 3) == c && c < (unsigned)s.m ? pr.ident : 0.f);
+            v[x] = __uint_as_float(pair_word(v[x]));
         }
-        if (in)
+        if (r < M && c < M)                              // (all 32 rows of a subtile or none)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) store4(out, lines, c, r + 8 * g, v + 4 * g);
+            for (int g = 0; g < 4; ++g) o.store(at, g, v + 4 * g);
     });
     if (mirror) t.store_rows(smem, out, lines, ti * BT, tj * BT, M, M);
 }
@@ -662,26 +692,26 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_apply(Batch b, int p, int t
     big_tile(blockIdx.x - s.first, (M + BT - 1) / BT, (N + BT - 1) / BT, ti, tj);
     Tile<C> t;
     t.run(smem, base + buffer_offset(p, s.m, s.n), M, base + buffer_offset(tin, s.m, s.n), N, M / LINE_K, ti * BT, tj * BT, 0, M / LINE_K);
-    char* const xo = base;
-    char* const to = base + buffer_offset(tout, s.m, s.n);
-    const char* const ti4 = base + buffer_offset(tin, s.m, s.n);
-    t.each([&](int row, int col, float* v) {
-        const unsigned r = ti * BT + row, c = tj * BT + col;
-        const bool in = r < M && c < N;
-        float old[16];
-        if (alpha != 0.f && in)
+    const Columns to = Columns::of(t, base + buffer_offset(tout, s.m, s.n), N, M / LINE_K, ti * BT, tj * BT);
+    const Columns from = Columns::of(t, base + buffer_offset(tin, s.m, s.n), N, M / LINE_K, ti * BT, tj * BT);
+    t.each([&](int row, int col, float* v, unsigned at) {
+        if (alpha != 0.f) {
+            float old[16];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) load4(ti4, M / LINE_K, c, r + 8 * g, old + 4 * g);
+            for (int g = 0; g < 4; ++g) from.load(at, g, old + 4 * g);
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-            v[x] *= scale;
-            if (alpha != 0.f && in) v[x] = fmaf(alpha, old[x], v[x]);
+            for (int x = 0; x < 16; ++x) v[x] = fmaf(alpha, old[x], v[x] * scale);
+        } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) v[x] *= scale;
         }
-        if (in)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) store4(to, M / LINE_K, c, r + 8 * g, v + 4 * g);
+        for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(pair_word(v[x]));
+        if (ti * BT + row < M && tj * BT + col < N)      // (all 32 rows of a subtile or none)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) to.store(at, g, v + 4 * g);
     });
-    t.store_rows(smem, xo, N / LINE_K, ti * BT, tj * BT, M, N);
+    t.store_rows(smem, base, N / LINE_K, ti * BT, tj * BT, M, N);
 }
 
 // the last product goes straight to where the caller wants it
@@ -726,15 +756,15 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_finish(TargetBatch b, Hyper
         keep = 1.f - lr * wd;
         step = lr * s.factor;
     }
-    const char* const old = s.turned ? base : T;         // row c of it, values r .. r+3: X's own order, or the other one
-    const unsigned old_lines = (s.turned ? N : M) / LINE_K;
-    t.each([&](int row, int col, float* v) {
+    // row c of it, values r .. r+3: X's own order, or the other one
+    const Columns old = Columns::of(t, s.turned ? base : T, s.turned ? M : N, (s.turned ? N : M) / LINE_K, r0, c0);
+    t.each([&](int row, int col, float* v, unsigned sub) {
         const unsigned c = c0 + col, r = r0 + row;
         if (c >= cols || r >= rows) return;              // (r is the lane's first row)
         if (b.alpha != 0.f) {
             float old4[16];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) load4(old, old_lines, c, r + 8 * g, old4 + 4 * g);    // padded rows: in the buffer
+            for (int g = 0; g < 4; ++g) old.load(sub, g, old4 + 4 * g);
 #pragma unroll
             for (int x = 0; x < 16; ++x) v[x] = fmaf(b.alpha, old4[x], v[x] * b.scale);
         } else {
