@@ -912,6 +912,12 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
+// Up to this many rows a rounding of A or Q is not averaged over many directions: it moves all singular values near 1, where the
+// terms of the polynomial cancel (0.7 = 3.44 - 4.77 + 2.03), ten times its size.  There A^2 and Q are taken in 64 bits and Q enters the product
+// as three fp16 numbers: median distance of 5 x 162 from 64-bit results 9.7e-7 -> 4.7e-7, of 16 x 200 8.2e-7 -> 4.6e-7 (the fp32 iteration
+// 6.9e-7, 6.6e-7), at no measurable time.
+constexpr int TINY = 16;
+
 template <int R>
 struct SmallShared {
     static constexpr int SUBS = R * (R + 1) / 2;         // 32 x 32 subtiles on and below the diagonal
@@ -922,6 +928,9 @@ struct SmallShared {
     } u;
     PairPlanes<R> A, Q;
     double red[8];
+    // R == 1, m <= TINY: A in 64 bits, and what Q's pairs leave of it
+    double a64[R == 1 ? TINY : 1][TINY + 1];
+    _Float16 rest[R == 1 ? 32 : 1][PairPlanes<R>::PITCH];
 };
 
 template <int R, int G, bool MUON>
@@ -936,6 +945,9 @@ __device__ __forceinline__ void small_matrix(const SmallBatch& b, const SmallIte
     const int slices = (n + 31) / 32, waves = slices < 8 ? slices : 8;
     const float mu = MUON ? (hd ? hd->mom[s.group] : h.mom[s.group]) : 0.f;
     const bool nest = MUON && b.nesterov;
+    const bool tiny = R == 1 && m <= TINY;
+    if (tiny)                                            // Q and its rest stay zero beyond the 16 rows and columns
+        for (int i = tid; i < 32 * PairPlanes<R>::PITCH; i += 512) (&Q.hi[0][0])[i] = (&Q.lo[0][0])[i] = (&sh.rest[0][0])[i] = (_Float16)0.f;
 
     // An element's byte offset is a lane's part (column, half of the rows) plus a uniform part (the row in the half): the instruction
     // adds the two.  A lane outside the matrix gets an offset beyond the buffer, which reads as 0 and drops what is written.
@@ -997,15 +1009,16 @@ __device__ __forceinline__ void small_matrix(const SmallBatch& b, const SmallIte
     if (lane == 0) red[wave] = sum;
     __syncthreads();
     const double norm = sqrt(((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7])));
-    int power;                                           // the factor may lie outside fp32's range: a number in [1/2, 1) and a power of two
-    const float factor = (float)frexp((double)b.scale / (norm <= b.eps ? b.eps : norm), &power);      // (a NaN norm stays)
+    // In 64 bits: the factor may lie outside fp32's range, and its rounding would be an error of all singular values at once, which the
+    // iteration enlarges tenfold near 1 (a NaN norm stays)
+    const double factor = (double)b.scale / (norm <= b.eps ? b.eps : norm);
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int p = 0; p < 8; ++p)
-                w[g][r][p].set(__builtin_amdgcn_ldexpf(x[g][r][2 * p] * factor, power), __builtin_amdgcn_ldexpf(x[g][r][2 * p + 1] * factor, power));
+                w[g][r][p].set((float)((double)x[g][r][2 * p] * factor), (float)((double)x[g][r][2 * p + 1] * factor));
 
     for (int step = 0; step < b.steps; ++step) {
         SmallStep k = b.step[step];
@@ -1062,12 +1075,37 @@ __device__ __forceinline__ void small_matrix(const SmallBatch& b, const SmallIte
                 }
                 const int ti = t == 0 ? 0 : 1, tj = t == 2 ? 1 : 0;
                 const int row = 32 * ti + 8 * e + 4 * (l >> 5), c = 32 * tj + (l & 31);
+                if (tiny) {
+                    if (row < TINY && c < TINY) {
+                        double d[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (i < waves) { d[0] += q[i].x; d[1] += q[i].y; d[2] += q[i].z; d[3] += q[i].w; }
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) sh.a64[row + x][c] = d[x] * k.gram;
+                    }
+                    continue;
+                }
                 const float a4[4] = {v.x * k.gram, v.y * k.gram, v.z * k.gram, v.w * k.gram};
                 A.store(row, c, a4, ti != tj);
             }
         }
         __syncthreads();
-        if (wave < SUBS) {   // Q = b A + c A^2, a wave per subtile
+        if (tiny) {          // Q = b A + c A^2, a thread per element
+            const int i = (tid >> 4) & 15, j = tid & 15;
+            if (tid < 256) {
+                double q = 0.0;
+#pragma unroll
+                for (int y = 0; y < TINY; ++y) q = fma(sh.a64[i][y], sh.a64[y][j], q);
+                q = fma(q, (double)k.quad, fma(sh.a64[i][j], (double)k.lin, i == j ? (double)k.ident : 0.0));
+                const _Float16 hi = (_Float16)(float)q;
+                const double left = q - (double)(float)hi;
+                const _Float16 lo = (_Float16)(float)left;
+                Q.hi[i][j] = hi;
+                Q.lo[i][j] = lo;
+                sh.rest[i][j] = (_Float16)(float)(left - (double)(float)lo);
+            }
+        } else if (wave < SUBS) {   // a wave per subtile
             const int ti = wave == 0 ? 0 : 1, tj = wave == 2 ? 1 : 0;
             f32x16 acc = zero16(), mix = zero16(), mix2 = zero16();
             PairFrag l[2 * R], r[2 * R];                 // all reads first
@@ -1099,6 +1137,11 @@ __device__ __forceinline__ void small_matrix(const SmallBatch& b, const SmallIte
             for (int r = 0; r < R; ++r) q[r] = Q.frag(32 * r + col, 16 * t + 4 * half, 16 * t + 8 + 4 * half);
         };
         q_block(0);
+        f16x8 rest = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (tiny) {
+            const uint2 a = *reinterpret_cast<const uint2*>(&sh.rest[col][4 * half]), b2 = *reinterpret_cast<const uint2*>(&sh.rest[col][8 + 4 * half]);
+            rest = __builtin_bit_cast(f16x8, make_uint4(a.x, a.y, b2.x, b2.y));
+        }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             if (g * 8 + wave >= slices) continue;
@@ -1113,6 +1156,7 @@ __device__ __forceinline__ void small_matrix(const SmallBatch& b, const SmallIte
                 for (int r = 0; r < R; ++r) now[r] = q[r];
                 q_block((t + 1) % (2 * R));
                 __builtin_amdgcn_sched_barrier(0);
+                if (t == 0 && tiny) acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rest, xf.hi, acc[0], 0, 0, 0);
 #pragma unroll
                 for (int r = 0; r < R; ++r) acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now[r].lo, xf.hi, acc[r], 0, 0, 0);
 #pragma unroll

@@ -632,7 +632,7 @@ def test_train_main_with_the_optimizer_from_config(cuda, tmp_path, name):
 
 def test_small_matrices_beside_large_ones_keep_the_callers_order(cuda):
     """Small matrices run on a stream of their own next to large ones: what the caller queued before a call, and what is queued behind it,
-    stay before and behind, on the default stream and on another, eager and captured."""
+    stay before and behind, on the default stream and on another."""
     gen = gen_of(cuda, 31)
     small, large = matrix("gauss", 30, 200, gen, cuda), matrix("gauss", 200, 900, gen, cuda)
     busy = torch.zeros(1 << 26, device=cuda)
@@ -650,3 +650,20 @@ def test_small_matrices_beside_large_ones_keep_the_callers_order(cuda):
                 assert torch.equal(x, want[0]) and torch.equal(y, want[1]), k
                 assert torch.equal(sums, want[0].sum() + want[1].sum())
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("r,c", [(2, 112), (5, 41), (162, 5), (7, 1000), (16, 200), (13, 2304)], ids=lambda v: str(v))
+def test_few_rows_are_closer_than_fp32(cuda, r, c):
+    """With few rows a rounding of A or Q moves all singular values at once, and near 1 the polynomial enlarges it tenfold (the terms of
+    0.7 = 3.44 - 4.77 + 2.03 cancel): that is most of the fp32 iteration's distance (2^-24 of each of A, b A, c A^2 and Q a step).  Here these are
+    in 64 bits and three fp16 numbers, and what is left are roundings of X, 2^-23 each at most, which are independent over r c entries.
+    Compared as root mean squares over 24 matrices, so that one unlucky spectrum decides nothing."""
+    gen = gen_of(cuda, 97 * r + c)
+    here = plain = 0.0
+    for _ in range(24):
+        m = matrix("gauss", r, c, gen, cuda)
+        want = iterate(m)
+        here += relative(optim.orthogonalize(m), want) ** 2
+        plain += relative(iterate(m, dtype=torch.float32), want) ** 2
+    print("%dx%d: %.2e, fp32 iteration %.2e" % (r, c, math.sqrt(here / 24), math.sqrt(plain / 24)))
+    assert here <= plain
