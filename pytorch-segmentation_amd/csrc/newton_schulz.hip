@@ -322,6 +322,12 @@ __global__ __launch_bounds__(256) void ns_normalise(SourceBatch b, Hyper h, cons
 // Per step: the wave waits for ITS copies of the step (those of STAGES - 2 later ones may be in flight), the barrier makes all waves'
 // visible and the step before it free, and the copies of the step STAGES - 1 ahead go there, one every few products: requested in one go the copies of
 // the waves keep each of them from issuing products for the 16 cycles a copy occupies the CU's address path.
+// What bounds a product: MFMA-bound it would take 384 cycles per 128 x 128 tile and line on a CU; LDS serves 32 KiB of reads and 16 KiB of
+// copies in about as many, L2 delivers those 16 KiB in 315 (its limit, 52 B a cycle and CU) to 680 (behind HBM), and the three meet: 800 - 900
+// cycles measured.  Short sums (m = 512 is 32 lines) add the tile's two stores, 128 KiB, at what HBM takes (4 TB/s).  512 x 36864: product
+// with P 92 us, of which 225 MB of HBM 50, the Gram product 38 us = 0.31 of the matrix rate.  Slower were: registers loaded a line ahead
+// (2 - 5 %), 64 x 64 tiles of 8 waves with half the lines each (10 %), both stores through LDS (7 - 10 %), five stages for two workgroups a CU
+// (0 - 3 %), tiles on XCDs in blocks (0).
 struct Wide { static constexpr int BT = 128, U = 1, PER_CU = 3; static constexpr unsigned STAGES = 3; };
 struct Many { static constexpr int BT = 64, U = 1, PER_CU = 4; static constexpr unsigned STAGES = 4; };
 struct Few { static constexpr int BT = 64, U = 2, PER_CU = 1; static constexpr unsigned STAGES = 8; };
@@ -1319,7 +1325,9 @@ unsigned tiles_of(int m, int bt) { return (pad64(m) + bt - 1) / bt; }
 unsigned low_tiles(int m, int bt) { const unsigned t = tiles_of(m, bt); return t * (t + 1) / 2; }
 unsigned big_tiles(const Shape& s, int bt) { return tiles_of(s.m, bt) * tiles_of(s.n, bt); }
 
-// Which tiles a launch runs on (see Tile)
+// Which tiles a launch runs on (see Tile).  128 x 128 copy half as much per product, 64 x 64 spread better: in us, WIDE / MANY, products of
+// m x m matrices with 408 tiles of 128 (3 of 2048 x 2048) 103 / 122, 288 (8 of 1024) 55 / 54, 257 (fifty filters) 34 / 31; with P 392 tiles
+// 27.7 / 29.7, 288 tiles 48 / 46.  Fewer 64s than CUs run one to a CU with a longer pipeline: 1024 x 1024 (136) 12.2 instead of 14.1.
 enum Config { WIDE, MANY, FEW };
 int tile_of(Config c) { return c == WIDE ? 128 : 64; }
 template <typename F>
@@ -1329,7 +1337,7 @@ Config config_of(const Shape* s, int count, F tiles) {
         wide += tiles(s[i], 128);
         many += tiles(s[i], 64);
     }
-    return wide >= SEGMI_NUM_CU ? WIDE : many > SEGMI_NUM_CU ? MANY : FEW;
+    return 4 * wide >= 5 * SEGMI_NUM_CU ? WIDE : many > SEGMI_NUM_CU ? MANY : FEW;
 }
 #define NS_LAUNCH(config, kernel, grid, ...)                                                                               \
     do {                                                                                                                   \
