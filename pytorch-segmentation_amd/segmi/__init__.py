@@ -2,7 +2,7 @@
 
     segmi.ops   functional ops + autograd glue (NHWC-backed tensors)
     segmi.nn    nn.Module subclasses with reference-compatible state_dict keys
-    segmi.optim fused multi-tensor SGD (torch.optim.SGD semantics and state layout)
+    segmi.optim fused multi-tensor SGD (torch.optim.SGD semantics and state layout), Muon, FusedAdamW, orthogonalize
     segmi.graph hipGraph capture / replay of a whole training step
 """
 from ._lib import LIB_PATH, SegmiError, lib  # noqa: F401  (raises if libsegmi.so is missing)
