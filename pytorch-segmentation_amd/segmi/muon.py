@@ -72,7 +72,7 @@ def orthogonalize(matrices, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
 
     `matrices`: a float32 or bfloat16 CUDA tensor of two or more dimensions (seen as shape[0] x the rest), or a list of them, any sizes
     and strides; all of them share the launches.  Returns new tensors of the same shapes, types and (where dense) strides.  Computed
-    to fp32 accuracy in both types.  No gradient is recorded.  A matrix that holds NaN or infinity comes back as NaN, a zero one as zero.
+    to fp32 accuracy in both types; the last bits may depend on what else is in the list.  No gradient is recorded.  A matrix that holds NaN or infinity comes back as NaN, a zero one as zero.
     Runs on the current stream of the tensors' device; may be captured into a hipGraph."""
     single = isinstance(matrices, torch.Tensor)
     mats = [matrices] if single else list(matrices)
@@ -186,9 +186,17 @@ class _FusedOptimizer(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As torch's, but the buffers are this optimizer's own: torch keeps the tensors of the dictionary where type and device fit,
         and the kernels here would advance those of the optimizer it came from as well.  Buffers that were there keep their place
-        and take the values, so a captured step goes on with what was loaded."""
+        and take the values, so a captured step goes on with what was loaded.  Settings that the dictionary lacks (another class wrote it) are
+        this optimizer's defaults; one that asks for a formula that is not here is refused."""
+        for g in state_dict["param_groups"]:
+            for key in ("amsgrad", "maximize"):
+                if g.get(key):
+                    raise ValueError("%s has no %s" % (self._name(), key))
         before = {p: dict(st) for p, st in self.state.items()}
         super().load_state_dict(state_dict)
+        for g in self.param_groups:
+            for key, value in self.defaults.items():
+                g.setdefault(key, value)
         with torch.no_grad():
             for p, st in self.state.items():
                 for key, v in st.items():

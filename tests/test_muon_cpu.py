@@ -172,3 +172,23 @@ def test_optimizers_copy_and_pickle():
             with pytest.raises((RuntimeError, AssertionError)):
                 opt.step()
             opt.load_state_dict(opt.state_dict())
+
+
+def test_loaded_settings():
+    p = [torch.nn.Parameter(torch.zeros(4, 4)), torch.nn.Parameter(torch.zeros(4))]
+    opt = optim.Muon(p, lr=0.5, adamw_lr_ratio=0.25)
+    sd = opt.state_dict()
+    for g in sd["param_groups"]:                     # as written by a class that knows less
+        for key in ("adamw_lr_ratio", "adamw_betas", "adamw_eps", "algorithm"):
+            del g[key]
+        g["lr"] = 0.125
+    opt.load_state_dict(sd)
+    g = opt.param_groups[0]
+    assert (g["lr"], g["adamw_lr_ratio"], g["adamw_betas"], g["algorithm"]) == (0.125, 0.25, (0.9, 0.95), "auto")
+    for key in ("amsgrad", "maximize"):
+        other = torch.optim.AdamW(p, lr=0.1, **{key: True})
+        with pytest.raises(ValueError, match=key):
+            optim.FusedAdamW(p).load_state_dict(other.state_dict())
+    mine = optim.FusedAdamW(p)
+    mine.load_state_dict(torch.optim.AdamW(p, lr=0.1, betas=(0.5, 0.6)).state_dict())
+    assert mine.param_groups[0]["lr"] == 0.1 and mine.param_groups[0]["betas"] == (0.5, 0.6)

@@ -667,3 +667,18 @@ def test_few_rows_are_closer_than_fp32(cuda, r, c):
         plain += relative(iterate(m, dtype=torch.float32), want) ** 2
     print("%dx%d: %.2e, fp32 iteration %.2e" % (r, c, math.sqrt(here / 24), math.sqrt(plain / 24)))
     assert here <= plain
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_orthogonalize_views_that_do_not_start_on_a_vector(cuda, dtype):
+    """Rows whose addresses are odd, for every class of sizes: the loads of four fall back to single ones."""
+    for r, c in ((7, 60), (40, 200), (100, 300), (130, 132)):
+        m = matrix("gauss", r, c, gen_of(cuda, r), cuda).to(dtype)
+        for v in (torch.zeros(r, c + 5, device=cuda, dtype=dtype)[:, 3:3 + c], torch.zeros(r * c + 1, device=cuda, dtype=dtype)[1:].view(r, c),
+                  torch.zeros(c, r + 3, device=cuda, dtype=dtype)[:, 2:2 + r].t()):
+            v.copy_(m)
+            out, want = optim.orthogonalize(v), iterate(m)
+            if dtype is torch.float32:
+                assert relative(out, want) <= 1e-5
+            else:
+                assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-4 * want.abs().max()).all())
