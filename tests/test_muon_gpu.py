@@ -682,3 +682,30 @@ def test_orthogonalize_views_that_do_not_start_on_a_vector(cuda, dtype):
                 assert relative(out, want) <= 1e-5
             else:
                 assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-4 * want.abs().max()).all())
+
+
+def test_orthogonalize_rows_gigabytes_apart(cuda):
+    """Offsets beyond 32 bits, in the source of a matrix that would otherwise be a small one, and of a larger one."""
+    store = torch.zeros(1_200_000_000, device=cuda)
+    for r, c, stride in ((20, 300, 60_000_000), (100, 300, 12_000_000), (1, 500, 7)):
+        m = matrix("gauss", r, c, gen_of(cuda, r), cuda)
+        for v in (torch.as_strided(store, (r, c), (stride, 1), 1), torch.as_strided(store, (c, r), (1, stride), 1)):
+            v.copy_(m if v.shape == m.shape else m.t())
+            assert relative(optim.orthogonalize(v), iterate(v)) <= 1e-5
+
+
+def test_fused_adamw_large_tensor_and_views(cuda):
+    """A tensor of more than 2^31 bytes beside a single number; parameters and gradients as views into one buffer."""
+    n = 600_000_000
+    flat, grads = torch.zeros(n + 5, device=cuda), torch.full((n + 5,), 1e-3, device=cuda)
+    flat[-3:] = 2.0
+    big, one = torch.nn.Parameter(flat[:n]), torch.nn.Parameter(flat[n + 4])
+    big.grad, one.grad = grads[:n], grads[n + 4]
+    opt = optim.FusedAdamW([big, one], lr=1e-2, weight_decay=0.0)
+    opt.step()
+    # the first step moves by lr g / (|g| + eps)
+    step = 1e-2 * 1e-3 / (1e-3 + 1e-8)
+    for at in (0, 1, n // 2, n - 1):
+        assert abs(float(flat[at]) + step) <= 8 * E24 * 1e-2, at
+    assert abs(float(flat[n + 4]) - (2.0 - step)) <= 4 * E24 * 2.0
+    assert flat[n:n + 4].tolist() == [0.0, 0.0, 2.0, 2.0]           # what lies between them is left alone
