@@ -240,8 +240,8 @@ class _FusedOptimizer(torch.optim.Optimizer):
 
     def _plan(self):
         """The step's descriptors.  They are made anew when anything they were made from is another: the parameters, which of them have
-        gradients, the groups' settings that enter them, a state tensor, any pointer or size.  (Addresses are compared, not objects alone:
-        `p.data = ...` keeps the object.)  The comparison is the host's share of a small step, so it runs over whole lists."""
+        gradients, the groups' settings that enter them, a parameter's state dictionary or a tensor in it, any pointer or size.  (Addresses are
+        compared, not objects alone: `p.data = ...` keeps the object.)  The comparison is the host's share of a small step, so it runs over whole lists."""
         flat = list(chain.from_iterable(map(_params, self.param_groups)))
         grads = [p.grad for p in flat]
         missing = [g is None for g in grads]
@@ -250,7 +250,8 @@ class _FusedOptimizer(torch.optim.Optimizer):
         if (k is not None and len(flat) == len(k["flat"]) and all(map(is_, flat, k["flat"])) and missing == k["missing"] and
                 list(map(_ptr, live)) == k["grad_ptrs"] and self._strides(flat, live, k["deep"], k["shallow"]) == k["strides"]):
             held = list(chain.from_iterable(map(dict.values, k["states"])))
-            if (len(held) == len(k["held"]) and all(map(is_, held, k["held"])) and list(map(_ptr, k["tensors"])) == k["ptrs"] and
+            if (all(map(is_, map(self.state.get, k["owners"]), k["states"])) and
+                    len(held) == len(k["held"]) and all(map(is_, held, k["held"])) and list(map(_ptr, k["tensors"])) == k["ptrs"] and
                     list(map(_numel, flat)) == k["numels"] and [p.shape for _, p in k["members"]] == k["shapes"] and
                     list(map(len, map(_params, self.param_groups))) == k["lengths"] and self._settings() == k["settings"]):
                 return k
@@ -271,13 +272,14 @@ class _FusedOptimizer(torch.optim.Optimizer):
         if rest:
             k["rest"] = self._adamw_descriptors(rest)
             k["rows"] = None if self.capturable else np.array([self._step_of[p] for _, p in rest])
-        states = [self.state[p] for _, p in mats + rest]
+        owners = [p for _, p in mats + rest]
+        states = [self.state[p] for p in owners]
         held = list(chain.from_iterable(map(dict.values, states)))
         tensors = flat + [t for st in states for key, t in st.items() if (key != "step" or self.capturable) and isinstance(t, torch.Tensor)]
         deep = [(i, j) for j, i in enumerate(i for i, g in enumerate(grads) if g is not None) if grads[i].dim() > 1]      # (among the parameters, among the gradients)
         shallow = [j for j, g in enumerate(live) if g.dim() == 1]
         k.update(flat=flat, missing=missing, grad_ptrs=list(map(_ptr, live)), deep=deep, shallow=shallow,
-                 strides=self._strides(flat, live, deep, shallow), states=states, held=held,
+                 strides=self._strides(flat, live, deep, shallow), owners=owners, states=states, held=held,
                  tensors=tensors, ptrs=list(map(_ptr, tensors)), numels=list(map(_numel, flat)), members=mats, shapes=[p.shape for _, p in mats],
                  lengths=list(map(len, map(_params, self.param_groups))), settings=self._settings())
         self._kept = k
