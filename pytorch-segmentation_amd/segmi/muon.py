@@ -168,9 +168,17 @@ class _FusedOptimizer(torch.optim.Optimizer):
 
     def add_param_group(self, group):
         super().add_param_group(group)
-        if len(self.param_groups) > _MAX_GROUPS:
+        try:
+            if len(self.param_groups) > _MAX_GROUPS:
+                raise ValueError("%s supports up to %d parameter groups" % (self._name(), _MAX_GROUPS))
+            self._check_group(self.param_groups[-1])         # completed from the defaults
+        except Exception:
             self.param_groups.pop()
-            raise ValueError("%s supports up to %d parameter groups" % (self._name(), _MAX_GROUPS))
+            raise
+
+    def _check_group(self, group):
+        """ValueError for settings that the kernels have no formula for."""
+        raise NotImplementedError
 
     def _name(self):
         return "segmi.optim." + type(self).__name__
@@ -187,11 +195,12 @@ class _FusedOptimizer(torch.optim.Optimizer):
         """As torch's, but the buffers are this optimizer's own: torch keeps the tensors of the dictionary where type and device fit,
         and the kernels here would advance those of the optimizer it came from as well.  Buffers that were there keep their place
         and take the values, so a captured step goes on with what was loaded.  Settings that the dictionary lacks (another class wrote it) are
-        this optimizer's defaults; one that asks for a formula that is not here is refused."""
+        this optimizer's defaults; one that asks for a formula that is not here, or holds settings the constructor would refuse, is refused."""
         for g in state_dict["param_groups"]:
             for key in ("amsgrad", "maximize"):
                 if g.get(key):
                     raise ValueError("%s has no %s" % (self._name(), key))
+            self._check_group({**self.defaults, **g})
         before = {p: dict(st) for p, st in self.state.items()}
         super().load_state_dict(state_dict)
         for g in self.param_groups:
@@ -392,6 +401,9 @@ class FusedAdamW(_FusedOptimizer):
         _check_common("segmi.optim.FusedAdamW", lr, weight_decay, betas, eps)
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay), capturable)
 
+    def _check_group(self, group):
+        _check_common(self._name(), group["lr"], group["weight_decay"], group["betas"], group["eps"])
+
     def _hyper_values(self):
         return [self._adamw_hyper("betas", "eps", None)]
 
@@ -426,6 +438,28 @@ def _matrix_of(p):
                        "strides %s" % (tuple(p.shape), tuple(p.stride())))
 
 
+def _check_muon(g):
+    name = "segmi.optim.Muon"
+    _check_common(name, g["lr"], g["weight_decay"], g["adamw_betas"], g["adamw_eps"])
+    if not 0.0 <= float(g["momentum"]) < 1.0:
+        raise ValueError("%s: momentum must be in [0, 1), got %r" % (name, g["momentum"]))
+    if not float(g["adamw_lr_ratio"]) >= 0.0:
+        raise ValueError("%s: invalid adamw_lr_ratio %r" % (name, g["adamw_lr_ratio"]))
+    _check_adjust(g["adjust_lr_fn"])
+    _check_algorithm(g["algorithm"])
+    _check_iteration(g["ns_steps"], g["ns_coefficients"], g["eps"], name)
+
+
+def _check_adjust(adjust_lr_fn):
+    if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
+        raise ValueError("segmi.optim.Muon: adjust_lr_fn must be None, 'original' or 'match_rms_adamw', got %r" % (adjust_lr_fn,))
+
+
+def _check_algorithm(algorithm):
+    if algorithm not in ("auto", "adamw"):
+        raise ValueError("segmi.optim.Muon: a group's algorithm is 'auto' or 'adamw', got %r" % (algorithm,))
+
+
 class Muon(_FusedOptimizer):
     """Momentum orthogonalised by Newton-Schulz products, for every parameter that is a matrix:
 
@@ -444,23 +478,15 @@ class Muon(_FusedOptimizer):
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=NS_COEFFICIENTS, eps=1e-7, ns_steps=5,
                  adjust_lr_fn=None, adamw_lr_ratio=1.0, adamw_betas=(0.9, 0.95), adamw_eps=1e-8, capturable=False):
-        _check_common("segmi.optim.Muon", lr, weight_decay, adamw_betas, adamw_eps)
-        if not 0.0 <= float(momentum) < 1.0:
-            raise ValueError("segmi.optim.Muon: momentum must be in [0, 1), got %r" % (momentum,))
-        if not float(adamw_lr_ratio) >= 0.0:
-            raise ValueError("segmi.optim.Muon: invalid adamw_lr_ratio %r" % (adamw_lr_ratio,))
-        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
-            raise ValueError("segmi.optim.Muon: adjust_lr_fn must be None, 'original' or 'match_rms_adamw', got %r" % (adjust_lr_fn,))
-        _check_iteration(ns_steps, ns_coefficients, eps, "segmi.optim.Muon")
+        _check_muon(dict(lr=lr, weight_decay=weight_decay, momentum=momentum, ns_coefficients=ns_coefficients, eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn,
+                         adamw_lr_ratio=adamw_lr_ratio, adamw_betas=adamw_betas, adamw_eps=adamw_eps, algorithm="auto"))
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=bool(nesterov),
                                       ns_coefficients=tuple(ns_coefficients), eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn,
                                       adamw_lr_ratio=adamw_lr_ratio, adamw_betas=tuple(adamw_betas), adamw_eps=adamw_eps, algorithm="auto"),
                          capturable)
 
-    def add_param_group(self, group):
-        if group.get("algorithm", "auto") not in ("auto", "adamw"):
-            raise ValueError("segmi.optim.Muon: a group's algorithm is 'auto' or 'adamw', got %r" % (group["algorithm"],))
-        super().add_param_group(group)
+    def _check_group(self, group):
+        _check_muon(group)
 
     def _hyper_values(self):
         h = np.zeros((3, _MAX_GROUPS), dtype=np.float32)
@@ -469,12 +495,16 @@ class Muon(_FusedOptimizer):
         return [h, self._adamw_hyper("adamw_betas", "adamw_eps", "adamw_lr_ratio")]
 
     def _is_matrix(self, group, p):
-        return group.get("algorithm", "auto") == "auto" and _matrix_of(p) is not None
+        algorithm = group.get("algorithm", "auto")
+        _check_algorithm(algorithm)
+        return algorithm == "auto" and _matrix_of(p) is not None
 
     def _settings(self):
         return [(g["adjust_lr_fn"], g.get("algorithm", "auto")) for g in self.param_groups]
 
     def _matrix_descriptors(self, members):
+        for gi in {gi for gi, _ in members}:
+            _check_adjust(self.param_groups[gi]["adjust_lr_fn"])
         rows = []
         for gi, p in members:
             g, (r, c) = self._checked(p), _matrix_of(p)

@@ -108,3 +108,43 @@ def test_a_reset_state_starts_anew(host, cls, reset):
         key = "momentum_buffer" if "momentum_buffer" in opt.state[p] else "exp_avg"
         if p.data_ptr() in pointers:
             assert pointers[p.data_ptr()] == opt.state[p][key].data_ptr()
+
+
+# ------------------------------------------------------------------------------------------------ groups
+BAD_SETTINGS = [(optim.Muon, key, value) for key, value in
+                (("adjust_lr_fn", "foo"), ("momentum", 1.5), ("momentum", -0.1), ("momentum", float("nan")), ("lr", -1.0), ("weight_decay", -0.1), ("adamw_betas", (0.9, 1.0)),
+                 ("adamw_betas", (0.9,)), ("adamw_eps", -1e-8), ("adamw_lr_ratio", -1.0), ("algorithm", "sgd"), ("ns_steps", 0), ("eps", 0.0),
+                 ("ns_coefficients", (9.0, 0.0, 0.0)))]
+BAD_SETTINGS += [(optim.FusedAdamW, key, value) for key, value in
+                 (("lr", -1.0), ("lr", float("nan")), ("weight_decay", -0.1), ("betas", (1.0, 0.9)), ("betas", (0.9, 0.9, 0.9)), ("eps", -1e-8))]
+
+
+@pytest.mark.parametrize("cls,key,value", BAD_SETTINGS, ids=lambda v: getattr(v, "__name__", str(v)))
+def test_a_groups_settings_are_checked(cls, key, value):
+    """What the constructor refuses as a default is refused in a group, in a group added later and in a loaded dictionary, which then
+    changes nothing."""
+    ps = parameters()
+    with pytest.raises(ValueError):
+        cls([{"params": ps[:1], key: value}])
+    opt = cls(ps[:2])
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": ps[2:], key: value})
+    assert len(opt.param_groups) == 1
+    before = opt.state_dict()
+    bad = opt.state_dict()
+    bad["param_groups"] = [dict(g, lr=0.125) for g in bad["param_groups"]]
+    bad["param_groups"][0][key] = value
+    with pytest.raises(ValueError):
+        opt.load_state_dict(bad)
+    assert opt.state_dict() == before
+    opt.add_param_group({"params": ps[2:], "lr": 0.5})
+    assert len(opt.param_groups) == 2
+
+
+@pytest.mark.parametrize("key,value", [("adjust_lr_fn", "foo"), ("algorithm", "AdamW")])
+def test_an_unknown_setting_made_later_is_refused(host, key, value):
+    opt = optim.Muon(parameters())
+    opt.step()
+    opt.param_groups[0][key] = value
+    with pytest.raises(ValueError, match=key):
+        opt.step()
