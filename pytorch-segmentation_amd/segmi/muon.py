@@ -200,6 +200,8 @@ class _FusedOptimizer(torch.optim.Optimizer):
             for key in ("amsgrad", "maximize"):
                 if g.get(key):
                     raise ValueError("%s has no %s" % (self._name(), key))
+            if g.get("decoupled_weight_decay") is False and g.get("weight_decay"):
+                raise ValueError("%s has decoupled weight decay only" % self._name())
             self._check_group({**self.defaults, **g})
         before = {p: dict(st) for p, st in self.state.items()}
         super().load_state_dict(state_dict)

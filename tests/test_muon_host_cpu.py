@@ -148,3 +148,16 @@ def test_an_unknown_setting_made_later_is_refused(host, key, value):
     opt.param_groups[0][key] = value
     with pytest.raises(ValueError, match=key):
         opt.step()
+
+
+# ------------------------------------------------------------------------------------------------ dictionaries of other classes
+@pytest.mark.parametrize("cls", OPTIMIZERS)
+def test_coupled_weight_decay_is_refused(cls):
+    """torch.optim.Adam adds the decay to the gradient, the formula here takes it off the parameter.  Without decay they are the same."""
+    ps = parameters()
+    opt = cls(ps)
+    with pytest.raises(ValueError, match="decoupled"):
+        opt.load_state_dict(torch.optim.Adam(ps, weight_decay=0.1).state_dict())
+    opt.load_state_dict(torch.optim.Adam(ps, lr=0.25, weight_decay=0.0).state_dict())
+    opt.load_state_dict(torch.optim.AdamW(ps, lr=0.25, weight_decay=0.1).state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["weight_decay"] == 0.1
