@@ -197,14 +197,16 @@ class _FusedOptimizer(torch.optim.Optimizer):
         and take the values, so a captured step goes on with what was loaded.  Settings that the dictionary lacks (another class wrote it) are
         this optimizer's defaults; one that asks for a formula that is not here, or holds settings the constructor would refuse, is refused."""
         for g in state_dict["param_groups"]:
-            for key in ("amsgrad", "maximize"):
+            for key in ("amsgrad", "maximize", "dampening"):
                 if g.get(key):
                     raise ValueError("%s has no %s" % (self._name(), key))
             if g.get("decoupled_weight_decay") is False and g.get("weight_decay"):
                 raise ValueError("%s has decoupled weight decay only" % self._name())
             self._check_group({**self.defaults, **g})
+        scales = [self._momentum_scale(g) for g in state_dict["param_groups"]]
         before = {p: dict(st) for p, st in self.state.items()}
         super().load_state_dict(state_dict)
+        scale_of = {p: s for g, s in zip(self.param_groups, scales) for p in g["params"]}
         for g in self.param_groups:
             for key, value in self.defaults.items():
                 g.setdefault(key, value)
@@ -218,7 +220,13 @@ class _FusedOptimizer(torch.optim.Optimizer):
                         st[key] = own.copy_(v)
                     else:
                         st[key] = v.clone()
+                    if key == "momentum_buffer" and scale_of.get(p, 1.0) != 1.0:
+                        st[key].mul_(scale_of[p])
         self._kept = None
+
+    def _momentum_scale(self, group):
+        """Factor that makes the momentum buffers of a dictionary's group sums, as they are here."""
+        return 1.0
 
     def _buffer(self, p, key):
         """state[p][key] in p's own memory order; created, or re-laid once if it arrived in another (a loaded state_dict)."""
@@ -472,7 +480,8 @@ class Muon(_FusedOptimizer):
     large as AdamW's, so one learning rate suits both halves), rows = shape[0].  Argument names follow torch.optim.Muon, which takes 2-D parameters
     only; this one takes a whole network: vectors, single rows and columns, depthwise filters and the parameters of groups
     with `"algorithm": "adamw"` are updated by AdamW with learning rate lr * adamw_lr_ratio, adamw_betas, adamw_eps and the group's weight_decay.
-    State: `momentum_buffer`, or `step`, `exp_avg`, `exp_avg_sq`.  Learning rate, weight decay, momentum and the AdamW
+    State: `momentum_buffer`, or `step`, `exp_avg`, `exp_avg_sq`.  torch.optim.Muon's buffer is a mean of the gradients, (1 - momentum) B: its
+    dictionaries are rescaled when they are loaded here, one of this class has to be before torch's loads it.  Learning rate, weight decay, momentum and the AdamW
     numbers may differ between groups (up to 8); nesterov, eps, ns_coefficients and ns_steps are one for all.  A parameter without gradient is
     left alone.  capturable=True: as segmi.optim.SGD."""
 
@@ -489,6 +498,11 @@ class Muon(_FusedOptimizer):
 
     def _check_group(self, group):
         _check_muon(group)
+
+    def _momentum_scale(self, group):
+        # torch.optim.Muon keeps a mean, buf.lerp_(grad, 1 - momentum); its groups have the iteration's settings and none for vectors
+        theirs = "ns_steps" in group and "adamw_lr_ratio" not in group
+        return 1.0 / (1.0 - float(group["momentum"])) if theirs else 1.0
 
     def _hyper_values(self):
         h = np.zeros((3, _MAX_GROUPS), dtype=np.float32)

@@ -161,3 +161,49 @@ def test_coupled_weight_decay_is_refused(cls):
     opt.load_state_dict(torch.optim.Adam(ps, lr=0.25, weight_decay=0.0).state_dict())
     opt.load_state_dict(torch.optim.AdamW(ps, lr=0.25, weight_decay=0.1).state_dict())
     assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["weight_decay"] == 0.1
+
+
+def test_momentum_of_torchs_muon_is_rescaled(host):
+    """torch.optim.Muon's buffer is a mean, buf.lerp_(grad, 1 - momentum); here it is a sum, 1 / (1 - momentum) times as large.  One
+    multiplication in fp32: half a step."""
+    p = torch.nn.Parameter(torch.zeros(80, 70))
+    theirs = torch.optim.Muon([{"params": [p], "momentum": 0.9}, {"params": [torch.nn.Parameter(torch.zeros(4, 6))]}], lr=0.0, weight_decay=0.0)
+    total = torch.zeros(80, 70, dtype=torch.float64)
+    gen = torch.Generator().manual_seed(3)
+    for _ in range(12):
+        p.grad = torch.randn(80, 70, generator=gen)
+        total = 0.9 * total + p.grad.double()
+        theirs.step()
+    sd = theirs.state_dict()
+    buf = theirs.state[p]["momentum_buffer"]
+    kept = buf.clone()
+    for warm in (False, True):                        # into an optimizer without state, and over the state of one
+        q = torch.nn.Parameter(torch.zeros(80, 70))
+        q.grad = torch.ones(80, 70)
+        opt = optim.Muon([{"params": [q]}, {"params": [torch.nn.Parameter(torch.zeros(4, 6))]}])
+        if warm:
+            opt.step()
+        opt.load_state_dict(sd)
+        got = opt.state[q]["momentum_buffer"]
+        assert torch.equal(buf, kept) and opt.param_groups[0]["momentum"] == 0.9
+        assert torch.allclose(got.double(), kept.double() / (1 - 0.9), rtol=2.0 ** -24 * 2, atol=0)
+        # torch's twelve steps: each rounds (1 - momentum) g, the difference and the sum, and the scale gives each back ten times as large
+        assert float((got.double() - total).abs().max()) <= 12 * 3 * 2.0 ** -24 * float(total.abs().max() + 10 * 5.0)
+        again = opt.state_dict()                      # its own dictionary is not rescaled
+        opt.load_state_dict(again)
+        assert torch.equal(opt.state[q]["momentum_buffer"], got)
+        other = optim.Muon([{"params": [torch.nn.Parameter(torch.zeros(80, 70))]}, {"params": [torch.nn.Parameter(torch.zeros(4, 6))]}])
+        other.load_state_dict(again)
+        assert torch.equal(other.state[other.param_groups[0]["params"][0]]["momentum_buffer"], got)
+
+
+def test_momentum_of_sgd_is_taken_as_it_is_and_dampened_sums_are_refused(host):
+    ps = parameters()
+    sgd = torch.optim.SGD(ps, lr=0.1, momentum=0.9)
+    for _ in range(2):
+        sgd.step()
+    opt = optim.Muon(ps)
+    opt.load_state_dict(sgd.state_dict())
+    assert torch.equal(opt.state[ps[0]]["momentum_buffer"], sgd.state[ps[0]]["momentum_buffer"])
+    with pytest.raises(ValueError, match="dampening"):
+        opt.load_state_dict(torch.optim.SGD(ps, lr=0.1, momentum=0.9, dampening=0.5).state_dict())
