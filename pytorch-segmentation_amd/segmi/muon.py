@@ -163,6 +163,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
         super().__init__(params, defaults)
         self.capturable = bool(capturable)
         self._hyper = None
+        self._where = None                           # see _device
         self._kept = None                            # what the last step saw and the descriptors made from it, see _plan
         self._steps, self._step_of, self._views = None, {}, []      # one flat host tensor of step numbers; state[p]["step"] are views of it
 
@@ -188,7 +189,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
 
     def __setstate__(self, state):                   # (torch's load_state_dict comes here too, with everything in place)
         super().__setstate__(state)
-        for name, value in (("capturable", False), ("_hyper", None), ("_kept", None), ("_steps", None), ("_step_of", {}), ("_views", [])):
+        for name, value in (("capturable", False), ("_hyper", None), ("_where", None), ("_kept", None), ("_steps", None), ("_step_of", {}), ("_views", [])):
             self.__dict__.setdefault(name, value)
 
     def load_state_dict(self, state_dict):
@@ -252,7 +253,12 @@ class _FusedOptimizer(torch.optim.Optimizer):
         return g
 
     def _device(self):
-        return self.param_groups[0]["params"][0].device
+        """Where the step runs: the device of the last step's first parameter with a gradient (groups may be empty, and what is frozen may lie
+        anywhere); before a step that of the first parameter on a GPU."""
+        if self._where is not None:
+            return self._where.device
+        params = list(chain.from_iterable(map(_params, self.param_groups)))
+        return next((p.device for p in params if p.is_cuda), params[0].device if params else None)
 
     def _is_matrix(self, group, p):
         return False
@@ -265,6 +271,8 @@ class _FusedOptimizer(torch.optim.Optimizer):
         grads = [p.grad for p in flat]
         missing = [g is None for g in grads]
         live = [g for g in grads if g is not None] if True in missing else grads
+        if live:
+            self._where = flat[missing.index(False)]
         k = self._kept
         if (k is not None and len(flat) == len(k["flat"]) and all(map(is_, flat, k["flat"])) and missing == k["missing"] and
                 list(map(_ptr, live)) == k["grad_ptrs"] and self._strides(flat, live, k["deep"], k["shallow"]) == k["strides"]):
@@ -354,10 +362,13 @@ class _FusedOptimizer(torch.optim.Optimizer):
             return
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("%s.push_hyper must stay outside the captured region (call it before graph replay)" % self._name())
+        device = self._device()
+        if device is None:
+            return
         values = np.concatenate([v.reshape(-1).view(np.uint8) for v in self._hyper_values()])
-        with _on(self._device()):
-            if self._hyper is None:
-                self._hyper = _Hyper(values.size, self._device())
+        with _on(device):
+            if self._hyper is None or self._hyper.dev.device != device:
+                self._hyper = _Hyper(values.size, device)
             self._hyper.push(values)
 
     def _ready(self):
@@ -365,7 +376,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
             if not self.capturable:
                 raise RuntimeError("%s: a step inside a hipGraph capture needs capturable=True (learning rates and step numbers would be "
                                    "frozen)" % self._name())
-            if self._hyper is None:
+            if self._hyper is None or self._hyper.dev.device != self._device():
                 raise RuntimeError("%s(capturable=True): run one eager step before capturing" % self._name())
         else:
             self.push_hyper()

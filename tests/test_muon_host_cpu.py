@@ -207,3 +207,21 @@ def test_momentum_of_sgd_is_taken_as_it_is_and_dampened_sums_are_refused(host):
     assert torch.equal(opt.state[ps[0]]["momentum_buffer"], sgd.state[ps[0]]["momentum_buffer"])
     with pytest.raises(ValueError, match="dampening"):
         opt.load_state_dict(torch.optim.SGD(ps, lr=0.1, momentum=0.9, dampening=0.5).state_dict())
+
+
+# ------------------------------------------------------------------------------------------------ which device
+@pytest.mark.parametrize("cls", OPTIMIZERS)
+def test_groups_without_parameters_and_without_gradients(host, cls):
+    """As torch.optim allows: an empty first group (everything in it frozen), no parameter at all, first parameters without a gradient."""
+    ps = parameters()
+    opt = cls([{"params": []}, {"params": ps}])
+    opt.step()
+    assert len(opt.state) == 3
+    cls([{"params": []}]).step()
+    held = torch.nn.Parameter(torch.zeros(3, device="meta"))              # elsewhere, and without a gradient
+    opt = cls([{"params": [held]}, {"params": ps}])
+    opt.step()
+    assert len(opt.state) == 3 and opt._device() == ps[0].device
+    empty = cls([{"params": []}], capturable=True)
+    empty.push_hyper()
+    empty.step()
