@@ -534,7 +534,7 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
  *     momentum = mu momentum + grad;   u = grad + mu momentum (nesterov) or momentum
  *     param = (1 - lr wd) param - lr factor orthogonalize(u)
  * lr, wd, mu per group (ngroups <= 8): host arrays, or, with hyper_dev, device memory in segmi_sgd_step_dev's layout (then the host
- * arrays are not read). */
+ * arrays are not read).  The updates run at the same time: no param or momentum may overlap another (nor may what segmi_adamw_step writes). */
 typedef struct segmi_muon_matrix {
     float* param;
     const float* grad;

@@ -299,6 +299,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
         if rest:
             k["rest"] = self._adamw_descriptors(rest)
             k["rows"] = None if self.capturable else np.array([self._step_of[p] for _, p in rest])
+        self._check_apart(k["mats"][0] if mats else None, k["rest"])
         owners = [p for _, p in mats + rest]
         states = [self.state[p] for p in owners]
         held = list(chain.from_iterable(map(dict.values, states)))
@@ -311,6 +312,25 @@ class _FusedOptimizer(torch.optim.Optimizer):
                  lengths=list(map(len, map(_params, self.param_groups))), settings=self._settings())
         self._kept = k
         return k
+
+    def _check_apart(self, mats, rest):
+        """Everything the kernels write lies in memory of its own: the updates of two tensors run at the same time."""
+        at, size = [], []
+        if mats is not None:
+            at += [mats["param"], mats["momentum"]]
+            size += [mats["rows"].astype(np.int64) * mats["cols"] * 4] * 2
+        if rest is not None:
+            at += [rest["param"], rest["exp_avg"], rest["exp_avg_sq"]]
+            size += [rest["count"] * 4] * 3
+            if self.capturable:
+                at.append(rest["step_dev"])
+                size.append(np.full(len(rest), 4))
+        if not at:
+            return
+        at, size = np.concatenate(at).astype(np.int64), np.concatenate(size)
+        order = np.argsort(at)
+        if np.any(at[order][:-1] + size[order][:-1] > at[order][1:]):
+            raise RuntimeError("%s: two of the parameters with gradients, or of their state buffers, share memory" % self._name())
 
     def _settings(self):
         return None

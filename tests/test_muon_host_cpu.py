@@ -225,3 +225,52 @@ def test_groups_without_parameters_and_without_gradients(host, cls):
     empty = cls([{"params": []}], capturable=True)
     empty.push_hyper()
     empty.step()
+
+
+# ------------------------------------------------------------------------------------------------ memory that two updates would write
+@pytest.mark.parametrize("cls", OPTIMIZERS)
+@pytest.mark.parametrize("shape", [(80, 70), (5600,)], ids=str)
+def test_parameters_that_share_memory_are_refused(host, cls, shape):
+    """One parameter twice, two parameters of one memory, overlapping views, one state buffer for two: their updates run at the same
+    time."""
+    def made(t):
+        p = torch.nn.Parameter(t)
+        p.grad = torch.ones_like(p)
+        return p
+
+    p = made(torch.zeros(shape))
+    flat = torch.zeros(3 * 5600)
+    near = made(flat[5600:11200].view(shape))
+    for other in (made(p.data), made(p.data.view(-1)), made(p.data.view(-1)[5599:])):
+        with pytest.raises(RuntimeError, match="share memory"):
+            cls([p, other]).step()
+        other.grad = None
+        cls([p, other]).step()                        # tied to one that is trained: not an update of its own
+    with pytest.raises(RuntimeError, match="share memory"):
+        cls([near, made(flat[11199:16799].view(shape))]).step()
+    cls([near, made(flat[:5600].view(shape)), made(flat[11200:].view(shape))]).step()           # neighbours
+    with pytest.warns(UserWarning, match="duplicate"):
+        twice = cls([p, p])
+    with pytest.raises(RuntimeError, match="share memory"):
+        twice.step()
+    q = made(torch.zeros(shape))
+    opt = cls([p, q])
+    opt.step()
+    key = next(k for k in opt.state[p] if k != "step")
+    opt.state[q][key] = opt.state[p][key]
+    with pytest.raises(RuntimeError, match="share memory"):
+        opt.step()
+    assert not host.calls or len(host.calls[-1][1])
+
+
+def test_a_refused_step_changes_no_step_numbers(host):
+    p = torch.nn.Parameter(torch.zeros(7))
+    q = torch.nn.Parameter(torch.zeros(7))
+    for t in (p, q):
+        t.grad = torch.ones(7)
+    opt = optim.FusedAdamW([p, q])
+    opt.step()
+    q.data = p.data
+    with pytest.raises(RuntimeError, match="share memory"):
+        opt.step()
+    assert float(opt.state[p]["step"]) == 1.0
