@@ -164,6 +164,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
         self.capturable = bool(capturable)
         self._hyper = None
         self._where = None                           # see _device
+        self._captured = []                          # what the graphs that hold a step of this optimizer point at
         self._kept = None                            # what the last step saw and the descriptors made from it, see _plan
         self._steps, self._step_of, self._views = None, {}, []      # one flat host tensor of step numbers; state[p]["step"] are views of it
 
@@ -189,13 +190,14 @@ class _FusedOptimizer(torch.optim.Optimizer):
 
     def __setstate__(self, state):                   # (torch's load_state_dict comes here too, with everything in place)
         super().__setstate__(state)
-        for name, value in (("capturable", False), ("_hyper", None), ("_where", None), ("_kept", None), ("_steps", None), ("_step_of", {}), ("_views", [])):
+        for name, value in (("capturable", False), ("_hyper", None), ("_where", None), ("_captured", []), ("_kept", None), ("_steps", None), ("_step_of", {}), ("_views", [])):
             self.__dict__.setdefault(name, value)
 
     def load_state_dict(self, state_dict):
         """As torch's, but the buffers are this optimizer's own: torch keeps the tensors of the dictionary where type and device fit,
         and the kernels here would advance those of the optimizer it came from as well.  Buffers that were there keep their place
-        and take the values, so a captured step goes on with what was loaded.  Settings that the dictionary lacks (another class wrote it) are
+        and take the values, so a captured step goes on with what was loaded; once a step was captured, those that the dictionary lacks
+        are set to zero in their place.  Settings that the dictionary lacks (another class wrote it) are
         this optimizer's defaults; one that asks for a formula that is not here, or holds settings the constructor would refuse, is refused."""
         for g in state_dict["param_groups"]:
             for key in ("amsgrad", "maximize", "dampening"):
@@ -212,11 +214,18 @@ class _FusedOptimizer(torch.optim.Optimizer):
             for key, value in self.defaults.items():
                 g.setdefault(key, value)
         with torch.no_grad():
+            if self._captured:
+                for p, st in before.items():
+                    for key, own in st.items():
+                        if isinstance(own, torch.Tensor) and self.state[p].get(key) is None:
+                            self.state[p][key] = own.zero_()
             for p, st in self.state.items():
                 for key, v in st.items():
                     if not isinstance(v, torch.Tensor):
                         continue
                     own = before.get(p, {}).get(key)
+                    if own is v:
+                        continue
                     if isinstance(own, torch.Tensor) and own.shape == v.shape and own.dtype == v.dtype and (own.device == v.device or key == "step"):
                         st[key] = own.copy_(v)
                     else:
@@ -391,13 +400,15 @@ class _FusedOptimizer(torch.optim.Optimizer):
                 self._hyper = _Hyper(values.size, device)
             self._hyper.push(values)
 
-    def _ready(self):
+    def _ready(self, k):
         if torch.cuda.is_current_stream_capturing():
             if not self.capturable:
                 raise RuntimeError("%s: a step inside a hipGraph capture needs capturable=True (learning rates and step numbers would be "
                                    "frozen)" % self._name())
             if self._hyper is None or self._hyper.dev.device != self._device():
                 raise RuntimeError("%s(capturable=True): run one eager step before capturing" % self._name())
+            # the graph's addresses stay valid for as long as the optimizer lives, whatever becomes of the state and the gradients
+            self._captured += [t.detach() for t in [*k["tensors"], *(p.grad for p in k["flat"] if p.grad is not None), self._hyper.dev]]
         else:
             self.push_hyper()
 
@@ -457,7 +468,7 @@ class FusedAdamW(_FusedOptimizer):
         k = self._plan()
         if k["rest"] is not None:
             with _on(self._device()):
-                self._ready()
+                self._ready(k)
                 self._adamw_launch(k, self._hyper_values()[0], self._hyper.dev.data_ptr() if self.capturable else None, torch.cuda.current_stream().cuda_stream)
         return loss
 
@@ -583,7 +594,7 @@ class Muon(_FusedOptimizer):
             return loss
         coef = _check_iteration(first["ns_steps"], first["ns_coefficients"], first["eps"], "segmi.optim.Muon")
         with _on(self._device()):
-            self._ready()
+            self._ready(k)
             hd = self._hyper.dev.data_ptr() if self.capturable else None
             h, a = self._hyper_values()
             stream = torch.cuda.current_stream().cuda_stream

@@ -274,3 +274,83 @@ def test_a_refused_step_changes_no_step_numbers(host):
     with pytest.raises(RuntimeError, match="share memory"):
         opt.step()
     assert float(opt.state[p]["step"]) == 1.0
+
+
+# ------------------------------------------------------------------------------------------------ what a captured step points at
+@pytest.fixture
+def capture(host, monkeypatch):
+    """capture(opt): one step as if a graph were being captured."""
+    class Hyper:
+        def __init__(self, nbytes, device):
+            self.dev = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+        def push(self, values):
+            pass
+
+    monkeypatch.setattr(muon, "_Hyper", Hyper)
+
+    def run(opt):
+        with monkeypatch.context() as m:
+            m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+            opt.step()
+    return run
+
+
+@pytest.mark.parametrize("cls", OPTIMIZERS)
+def test_a_captured_steps_buffers_outlive_a_load_without_state(host, capture, cls):
+    """A graph holds addresses: a dictionary without state (a new optimizer's) sets the buffers to zero where they are, and buffers that
+    leave the state stay allocated."""
+    ps = parameters()
+    opt = cls(ps, lr=0.5, capturable=True)
+    opt.step()
+    capture(opt)
+    captured = host.calls[-1][1].copy()
+    buffers = {p: dict(opt.state[p]) for p in ps}
+    for st in buffers.values():
+        for v in st.values():
+            v.fill_(3.0)
+    opt.load_state_dict(cls(parameters(), lr=0.25).state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25
+    for p in ps:
+        assert opt.state[p].keys() == buffers[p].keys()
+        for key, v in opt.state[p].items():
+            assert v is buffers[p][key] and not v.any(), key
+    opt.step()
+    assert all(np.array_equal(host.calls[-1][1][f], captured[f]) for f in captured.dtype.names)
+
+
+@pytest.mark.parametrize("cls", OPTIMIZERS)
+def test_a_captured_steps_memory_is_kept(host, capture, cls):
+    import gc
+    import weakref
+    ps = parameters()
+    opt = cls(ps, capturable=True)
+    opt.step()
+    storages = lambda: [t.untyped_storage().data_ptr() for p in ps for t in [p, p.grad, *opt.state[p].values()]]
+    before = storages()
+    capture(opt)
+    held = {t.untyped_storage().data_ptr() for t in opt._captured}
+    assert held.issuperset(before)
+    watched = [weakref.ref(t) for t in opt._captured]
+    opt.state.clear()
+    for p in ps:
+        p.data = p.data.clone()
+        p.grad = None
+        p.grad = torch.ones_like(p)
+    opt.step()
+    gc.collect()
+    assert all(w() is not None for w in watched)
+    assert not set(storages()) & set(before)             # the eager step has buffers of its own
+    import copy
+    assert copy.deepcopy(opt)._captured == []
+
+
+@pytest.mark.parametrize("cls", OPTIMIZERS)
+def test_a_load_without_state_and_without_a_graph_leaves_none(host, cls):
+    ps = parameters()
+    opt = cls(ps)
+    opt.step()
+    opt.load_state_dict(cls(parameters()).state_dict())
+    assert not opt.state_dict()["state"]
+    opt.step()
+    assert all(float(st["step"]) == 1.0 for st in opt.state.values() if "step" in st)

@@ -26,3 +26,34 @@ def test_reset_state_steps_like_a_new_optimizer(cuda, cls, capturable):
             assert torch.equal(p, q)
             assert a.state[p].keys() == b.state[q].keys()
             assert all(torch.equal(torch.as_tensor(a.state[p][n]), torch.as_tensor(v)) for n, v in b.state[q].items())
+
+
+@pytest.mark.parametrize("cls", ["Muon", "FusedAdamW"])
+def test_captured_step_after_a_load_without_state(cuda, cls):
+    """A new optimizer's dictionary starts a captured step anew, in the buffers the graph points at."""
+    ps, qs = network(cuda, 14), network(cuda, 14)
+    make = lambda ts: getattr(optim, cls)(ts, lr=1e-2, capturable=True)
+    a = make(ps)
+    a.step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a.step()
+    g.replay()
+    a.load_state_dict(make(qs).state_dict())
+    churn = [torch.randn(4096, device=cuda) for _ in range(64)]          # whatever was freed has other contents now
+    for p, q in zip(ps, qs):
+        q.data.copy_(p)
+    b = make(qs)
+    for k in range(3):
+        for p, q in zip(ps, qs):
+            n = torch.randn_like(p)
+            p.grad.copy_(n)
+            q.grad.copy_(n)
+        a.push_hyper()
+        g.replay()
+        b.step()
+        torch.cuda.synchronize()
+        for i, (p, q) in enumerate(zip(ps, qs)):
+            assert torch.equal(p, q), (k, i)
+            assert all(torch.equal(a.state[p][n], v) for n, v in b.state[q].items()), (k, i)
+    del churn
