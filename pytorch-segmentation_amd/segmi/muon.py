@@ -94,6 +94,9 @@ def orthogonalize(matrices, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
             device, index = t.device, t.get_device()
         elif t.get_device() != index:
             raise SegmiError("segmi.optim.orthogonalize: all matrices must be on one device, got %s and %s" % (device, t.device))
+        if t.is_neg():                            # memory holds the opposite sign (the imaginary part of a conjugate)
+            t = t.resolve_neg()
+            keep.append(t)
         out = torch.empty_like(t)
         n = t.numel()
         if n and t.dim() == 2:
@@ -257,6 +260,8 @@ class _FusedOptimizer(torch.optim.Optimizer):
         if not (p.is_cuda and p.dtype == torch.float32 and not g.is_sparse and g.dtype == torch.float32 and g.device == p.device and
                 _same_layout(g, p) and _unit_of(p.shape, p.stride()) == 1):
             raise RuntimeError("%s: parameters and gradients must be float32 CUDA tensors on one device with identical (dense) strides" % self._name())
+        if p.is_neg() or g.is_neg():
+            raise RuntimeError("%s: a parameter or gradient is a negated view; resolve_neg() makes one the kernels can read" % self._name())
         if p.device != self._device():
             raise RuntimeError("%s: all parameters must be on one device, got %s and %s" % (self._name(), self._device(), p.device))
         return g

@@ -57,3 +57,16 @@ def test_captured_step_after_a_load_without_state(cuda, cls):
             assert torch.equal(p, q), (k, i)
             assert all(torch.equal(a.state[p][n], v) for n, v in b.state[q].items()), (k, i)
     del churn
+
+
+def test_negated_views_are_what_they_stand_for(cuda):
+    """The imaginary part of a conjugate is a view whose memory holds the opposite sign."""
+    z = torch.randn(40, 70, dtype=torch.complex64, device=cuda)
+    view = z.conj().imag
+    assert view.is_neg()
+    assert torch.equal(optim.orthogonalize(view), optim.orthogonalize((-z.imag).contiguous()))
+    p = torch.nn.Parameter(torch.zeros(40, 70, device=cuda))
+    p.grad = torch._neg_view(torch.ones(40, 70, device=cuda))
+    for cls in (optim.Muon, optim.FusedAdamW):
+        with pytest.raises(RuntimeError, match="negated"):
+            cls([p]).step()
