@@ -22,6 +22,8 @@
 //
 // Symmetric products compute the tiles on and below the diagonal and store each twice.
 //
+// Up to 16 rows are another matter (see TINY): small_matrix and ns_thin take their Gram matrix and Q in 64 bits.
+//
 // Layout.  A line is 16 consecutive values of a row as 16 fp16 hi followed by 16 fp16 lo, 64 bytes: one matrix instruction's K, one
 // DMA row of LDS.  64 rows form a panel, in which line q of all 64 rows is one 4 KiB run, so that what a workgroup requests per step is
 // contiguous.  Both dimensions are padded to 64 with zeros: no kernel but the first and the last knows a border.
@@ -809,7 +811,7 @@ __global__ __launch_bounds__(256, C::PER_CU) void ns_finish(TargetBatch b, Hyper
 //     X <- a X + Q X    X goes into the instruction as it lies in the registers: the sum over rows may run in any order, so Q's words
 //                       are read in the order in which a lane holds the rows
 // Bound by latency: 64 x 576 is 25 MFLOP a step on one CU (2.7 us at its peak rate) plus four barriers.
-enum Class { SMALL_1_1, SMALL_1_3, SMALL_1_9, SMALL_2_1, SMALL_2_3, SQUARE, WIDE_MATRIX, CLASSES };    // SMALL_R_G
+enum Class { SMALL_1_1, SMALL_1_3, SMALL_1_9, SMALL_2_1, SMALL_2_3, THIN, SQUARE, WIDE_MATRIX, CLASSES };    // SMALL_R_G
 struct SmallItem {
     const void* src;                 // MUON: the gradient
     void* dst;                       // MUON: the parameter
@@ -1226,6 +1228,161 @@ __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const 
     }
 }
 
+// ------------------------------------------------------------------------------------------------ thin matrices
+// Up to TINY rows that small_matrix does not take (more than 2304 columns, or a span beyond its 32-bit offsets).  For the reason given at TINY
+// the Gram matrix, A^2, Q and the products with Q are all taken in 64 bits; X is held in fp32, [row][column].  A launch per step: a workgroup adds
+// the Gram matrix's parts, one per workgroup of the launch before, in their order, makes Q of them, takes its columns through
+// X <- (a I + b A + c A^2) X, one column a thread, and leaves its part of the new Gram matrix, one element a thread.
+// Distance from 64-bit results (root mean square of 16 matrices): 16 x 4608 6e-8, noise with strong directions 1.6e-7; as fp16 pairs through the
+// products above 1.3e-6, the fp32 iteration 1.0e-6.  Time, here / there: 3 x 5000 57 / 94 us, 16 x 36864 113 / 152, 16 x 10^6 656 / 1046, 32 of
+// 8 x 10000 168 / 358; 16 x 4608 beside 256 x 1024, which it no longer shares launches with, 188 / 134, beside a network's filters nothing.
+// Bound by latency up to some 10^5 columns (seven launches), then by LDS, which serves two fp32 operands of every 64-bit product (16 x 16 000 000:
+// 8.6 ms for 12 GB of X, 1.4 TB/s).
+struct ThinItem {
+    const void* src;                 // MUON: the gradient
+    void* dst;                       // MUON: the parameter
+    float* mom;
+    long si, sj, di, dj;             // strides of X's rows and columns in src (and mom), and in dst
+    size_t x;                        // X in the batch's X region
+    unsigned first;                  // first workgroup of a launch; also the first part of the Gram matrix
+    unsigned part, parts;            // its partial sums of squares
+    int m, n;
+    float factor;                    // MUON
+    short dtype, group;
+};
+constexpr int THIN_BATCH = 32;
+struct ThinBatch {
+    float* x;
+    const double* partial;
+    double* gram[2];                 // parts of 256 values, read and written in turns
+    double a, b, c, eps;
+    int count, nesterov;
+    ThinItem item[THIN_BATCH];
+};
+static_assert(sizeof(ThinBatch) + sizeof(Hyper) + 2 * sizeof(void*) < 4096, "kernel arguments");
+constexpr int THIN_TILE = 256;       // columns at a time
+// Columns per workgroup: at most 256 workgroups a matrix, so that adding their parts stays short.
+__host__ __device__ inline unsigned thin_columns(int n) { return THIN_TILE * (((unsigned)n + 256u * THIN_TILE - 1) / (256u * THIN_TILE)); }
+__host__ __device__ inline unsigned thin_groups(int n) { return ((unsigned)n + thin_columns(n) - 1) / thin_columns(n); }
+
+enum ThinStage { THIN_FIRST, THIN_NEXT, THIN_LAST };     // source to X; X to X; X to the destination
+
+template <int STAGE, bool MUON>
+__global__ __launch_bounds__(256) void ns_thin(ThinBatch b, int from, Hyper h, const Hyper* __restrict__ hd) {
+    __shared__ double red[4];
+    __shared__ double gram[TINY][TINY + 1], q[TINY][TINY];
+    __shared__ __attribute__((aligned(16))) float tile[TINY][THIN_TILE + 4];        // ds_read_b128 of 16 rows covers all 64 banks
+    const ThinItem s = b.item[find_item(b, blockIdx.x)];
+    const int tid = threadIdx.x, gi = tid >> 4, gj = tid & 15;
+    const unsigned part = blockIdx.x - s.first, groups = thin_groups(s.n), cols = thin_columns(s.n);
+    const size_t pitch = pad64(s.n);
+    float* const x = b.x + s.x;
+    double inv = 0.0;
+    if (STAGE == THIN_FIRST) {
+        double sum = 0.0;
+        for (unsigned i = tid; i < s.parts; i += 256) sum += b.partial[s.part + i];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if ((tid & 63) == 0) red[tid >> 6] = sum;
+        __syncthreads();
+        const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
+        inv = 1.0 / (norm <= b.eps ? b.eps : norm);      // (a NaN norm stays)
+    } else {
+        const double* const in = b.gram[from] + (size_t)s.first * 256 + tid;
+        double v = 0.0;
+#pragma unroll 8
+        for (unsigned g = 0; g < groups; ++g) v += in[(size_t)g * 256];
+        gram[gi][gj] = v;
+        __syncthreads();
+        double sq = 0.0;
+#pragma unroll
+        for (int y = 0; y < TINY; ++y) sq = fma(gram[gi][y], gram[y][gj], sq);
+        q[gi][gj] = fma(b.c, sq, fma(b.b, v, gi == gj ? b.a : 0.0));
+        __syncthreads();
+    }
+    const float mu = MUON ? (hd ? hd->mom[s.group] : h.mom[s.group]) : 0.f;
+    const bool nest = MUON && b.nesterov;
+    float keep = 1.f, rate = 0.f;
+    if (MUON && STAGE == THIN_LAST) {
+        const float lr = hd ? hd->lr[s.group] : h.lr[s.group], wd = hd ? hd->wd[s.group] : h.wd[s.group];
+        keep = 1.f - lr * wd;
+        rate = lr * s.factor;
+    }
+    double acc = 0.0;
+    const unsigned end = part * cols + cols < (unsigned)s.n ? part * cols + cols : (unsigned)s.n;
+#pragma unroll 1
+    for (unsigned c0 = part * cols; c0 < end; c0 += THIN_TILE) {
+        const unsigned col = c0 + tid;
+        const bool in = col < end;
+        float v[TINY];
+#pragma unroll
+        for (int r = 0; r < TINY; ++r) v[r] = 0.f;
+        if (in) {                                        // all loads first
+#pragma unroll
+            for (int r = 0; r < TINY; ++r) {
+                if (r >= s.m) continue;
+                if (STAGE != THIN_FIRST) {
+                    v[r] = x[r * pitch + col];
+                    continue;
+                }
+                const long off = (long)r * s.si + (long)col * s.sj;
+                const float g = !MUON || nest ? (s.dtype ? bf16_to_f32(static_cast<const unsigned short*>(s.src)[off]) : static_cast<const float*>(s.src)[off]) : 0.f;
+                const float m = MUON ? s.mom[off] : 0.f;             // already advanced
+                v[r] = !MUON ? g : nest ? fmaf(mu, m, g) : m;
+            }
+        }
+        if (STAGE == THIN_FIRST) {
+#pragma unroll
+            for (int r = 0; r < TINY; ++r)
+                if (in && r < s.m) v[r] = (float)((double)v[r] * inv);
+        } else {
+            double w[TINY];
+#pragma unroll
+            for (int r = 0; r < TINY; ++r) {
+                w[r] = 0.0;
+                if (r >= s.m) continue;
+#pragma unroll
+                for (int k = 0; k < TINY; ++k) w[r] = fma(q[r][k], (double)v[k], w[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < TINY; ++r) v[r] = in ? (float)w[r] : 0.f;
+        }
+        if (STAGE == THIN_LAST) {
+            if (!in) continue;
+#pragma unroll
+            for (int r = 0; r < TINY; ++r) {
+                if (r >= s.m) continue;
+                const long off = (long)r * s.di + (long)col * s.dj;
+                if (MUON) {
+                    float* const p = static_cast<float*>(s.dst) + off;
+                    *p = fmaf(-rate, v[r], *p * keep);
+                } else if (s.dtype) {
+                    static_cast<unsigned short*>(s.dst)[off] = f32_to_bf16(v[r]);
+                } else {
+                    static_cast<float*>(s.dst)[off] = v[r];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < TINY; ++r) {
+                if (in && r < s.m) x[r * pitch + col] = v[r];
+                tile[r][tid] = v[r];
+            }
+            __syncthreads();
+            if (gi < s.m && gj < s.m)
+                for (int k = 0; k < THIN_TILE; k += 4) {
+                    const float4 l = *reinterpret_cast<const float4*>(&tile[gi][k]), r = *reinterpret_cast<const float4*>(&tile[gj][k]);
+                    acc = fma((double)l.x, (double)r.x, acc);
+                    acc = fma((double)l.y, (double)r.y, acc);
+                    acc = fma((double)l.z, (double)r.z, acc);
+                    acc = fma((double)l.w, (double)r.w, acc);
+                }
+            __syncthreads();
+        }
+    }
+    if (STAGE != THIN_LAST) b.gram[STAGE == THIN_FIRST ? from : 1 - from][(size_t)(s.first + part) * 256 + tid] = acc;
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 // Largest value of |f| on [0, s] for the polynomials of the iteration, and the power-of-two scale that keeps such entries below 2^15
 // (fp16 ends at 65504; a matrix's entries are bounded by its spectral norm).
@@ -1288,6 +1445,7 @@ Class class_of(int rows, int cols, size_t span) {
         if (m <= 32 && n <= 2304) return n <= 256 ? SMALL_1_1 : n <= 768 ? SMALL_1_3 : SMALL_1_9;
         if (m <= 64 && n <= 768) return n <= 256 ? SMALL_2_1 : SMALL_2_3;
     }
+    if (m <= TINY) return THIN;
     return is_wide(m, n) ? WIDE_MATRIX : SQUARE;
 }
 size_t span_of(const segmi_ns_matrix& a) {
@@ -1521,6 +1679,64 @@ int run_batch(bool wide, const Shape* shapes, SourceBatch& src, TargetBatch& dst
     return segmi_launch_status();
 }
 
+struct ThinPlan {
+    size_t gram_at, x_at, bytes;
+    unsigned groups;
+};
+ThinPlan thin_plan(const Shape* s, int count) {
+    ThinPlan p{};
+    size_t parts = 0, x = 0;
+    for (int i = 0; i < count; ++i) {
+        parts += (size_t)segmi_cdiv(s[i].outer, 64) * segmi_cdiv(s[i].inner, 256);
+        p.groups += thin_groups(s[i].n);
+        x += (size_t)s[i].m * pad64(s[i].n);
+    }
+    p.gram_at = align256(parts * sizeof(double));
+    p.x_at = p.gram_at + 2 * (size_t)p.groups * 256 * sizeof(double);
+    p.bytes = p.x_at + x * sizeof(float);
+    return p;
+}
+
+// `src` and `dst` carry the callers' pointers, as in run_batch
+template <bool MUON>
+int run_thin(const Shape* shapes, SourceBatch& src, const TargetBatch& dst, int count, const Bounds& f, int steps, char* ws, const Hyper& h,
+             const Hyper* hd, hipStream_t st) {
+    const ThinPlan plan = thin_plan(shapes, count);
+    src.ws = ws;
+    src.partial = reinterpret_cast<double*>(ws);
+    src.count = count;
+    ThinBatch b{};
+    b.x = reinterpret_cast<float*>(ws + plan.x_at);
+    b.partial = src.partial;
+    b.gram[0] = reinterpret_cast<double*>(ws + plan.gram_at);
+    b.gram[1] = b.gram[0] + (size_t)plan.groups * 256;
+    b.a = f.a;
+    b.b = f.b;
+    b.c = f.c;
+    b.eps = src.eps;
+    b.count = count;
+    b.nesterov = src.nesterov;
+    unsigned g_sum = 0, grid = 0;
+    size_t x = 0;
+    for (int i = 0; i < count; ++i) {
+        const Shape& s = shapes[i];
+        Source& o = src.item[i];
+        const Target& t = dst.item[i];
+        o.first = o.part = g_sum;
+        o.parts = segmi_cdiv(s.outer, 64) * segmi_cdiv(s.inner, 256);
+        b.item[i] = ThinItem{o.src, t.dst, o.mom, o.inner_is_n ? o.so : o.si, o.inner_is_n ? o.si : o.so, t.si, t.sj, x, grid, o.part, o.parts,
+                             s.m, s.n, t.factor, (short)t.dtype, (short)t.group};
+        g_sum += o.parts;
+        grid += thin_groups(s.n);
+        x += (size_t)s.m * pad64(s.n);
+    }
+    hipLaunchKernelGGL((ns_sum_squares<MUON>), dim3(g_sum), dim3(256), 0, st, src, h, hd);
+    hipLaunchKernelGGL((ns_thin<THIN_FIRST, MUON>), dim3(grid), dim3(256), 0, st, b, 0, h, hd);
+    for (int i = 0; i + 1 < steps; ++i) hipLaunchKernelGGL((ns_thin<THIN_NEXT, MUON>), dim3(grid), dim3(256), 0, st, b, i & 1, h, hd);
+    hipLaunchKernelGGL((ns_thin<THIN_LAST, MUON>), dim3(grid), dim3(256), 0, st, b, (steps - 1) & 1, h, hd);
+    return segmi_launch_status();
+}
+
 // `b` carries the callers' pointers; the steps' scales are filled in here
 template <bool MUON>
 int run_small(SmallBatch& b, int count, const Bounds& f, int steps, const Hyper& h, const Hyper* hd, hipStream_t st) {
@@ -1550,7 +1766,7 @@ int run_small(SmallBatch& b, int count, const Bounds& f, int steps, const Hyper&
     return segmi_launch_status();
 }
 
-// Small matrices take one CU each for as long as a third of a network's whole step, so next to others they run on a stream of
+// Small matrices take one CU each for as long as a third of a network's whole step, so next to others they run (and thin ones with them) on a stream of
 // their own, which waits for the caller's and is waited for by it (a whole Muon step of PSPNet's filters 1777 -> 1728 us, of UNet's 1194 -> 1130;
 // five small ones beside 150 x 257 and 333 x 65 242 -> 210 us for a call alone.  The two waits cost the host 25 us.)
 // Inside a capture everything stays on the captured stream: this one may be at work for another thread.
@@ -1598,7 +1814,7 @@ public:
 template <typename M>
 bool mixed(const M* mats, int count) {
     int small = 0;
-    for (int i = 0; i < count; ++i) small += class_of(mats[i]) < SQUARE;
+    for (int i = 0; i < count; ++i) small += class_of(mats[i]) < THIN;
     return small && small < count;
 }
 
@@ -1618,9 +1834,9 @@ Shape shape_of(const segmi_ns_matrix& a) { return shape_of(a.rows, a.cols, a.src
 // 441 / 455.
 constexpr size_t JOIN_WORK = (size_t)1 << 32;            // sum of m^2 n
 
-// The matrices of a call in batches of one kind (small, square, wide), those with the longest sums first (what is started last should be short):
-// f(class, indices, how many) in order, until it returns something other than SEGMI_OK.  Batches run one after the other and share
-// the workspace.
+// The matrices of a call in batches of one kind (small, thin, square, wide), those with the longest sums first (what is started last should be short):
+// f(class, indices, how many) in order, until it returns something other than SEGMI_OK.  Batches of one stream run one after the other and
+// share their part of the workspace.
 template <typename M, typename F>
 int for_batches(const M* mats, int count, F f) {
     const auto side = [&](int i) { return mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols; };
@@ -1640,7 +1856,7 @@ int for_batches(const M* mats, int count, F f) {
             if ((join && own == WIDE_MATRIX ? SQUARE : own) == c) order[k++] = i;
         }
         std::sort(order.get(), order.get() + k, [&](int a, int b) { return side(a) != side(b) ? side(a) > side(b) : a < b; });
-        const int most = c < SQUARE ? SMALL_BATCH : BATCH;
+        const int most = c < THIN ? SMALL_BATCH : c == THIN ? THIN_BATCH : BATCH;
         for (int at = 0; at < k; at += most) {
             const int rc = f((Class)c, order.get() + at, k - at < most ? k - at : most);
             if (rc != SEGMI_OK) return rc;
@@ -1649,19 +1865,26 @@ int for_batches(const M* mats, int count, F f) {
     return SEGMI_OK;
 }
 
+// The workspace: `thin` bytes that the thin batches share, which may run beside the others, and `rest` that those share.
+struct Need {
+    size_t thin, rest;
+    size_t bytes() const { return rest ? thin + rest : 0; }
+};
 template <typename M, typename F>
-size_t workspace_of(const M* mats, int count, F shape) {
-    size_t most = 256;                                   // (small matrices need none; 0 means refused)
+Need need_of(const M* mats, int count, F shape) {
+    Need need{0, 256};                                   // (small matrices need none; 0 means refused)
     const int rc = for_batches(mats, count, [&](Class c, const int* index, int k) {
-        if (c < SQUARE) return (int)SEGMI_OK;
+        if (c < THIN) return (int)SEGMI_OK;
         Shape s[BATCH];
         for (int i = 0; i < k; ++i) s[i] = shape(mats[index[i]]);
-        const Plan p = plan_batch(s, k);
-        if (p.bytes > most) most = p.bytes;
+        if (c == THIN) need.thin = std::max(need.thin, align256(thin_plan(s, k).bytes));
+        else need.rest = std::max(need.rest, plan_batch(s, k).bytes);
         return (int)SEGMI_OK;
     });
-    return rc == SEGMI_OK ? most : 0;
+    return rc == SEGMI_OK ? need : Need{0, 0};
 }
+Need need_of(const segmi_ns_matrix* mats, int count) { return need_of(mats, count, [](const segmi_ns_matrix& a) { return shape_of(a); }); }
+Need need_of(const segmi_muon_matrix* mats, int count) { return need_of(mats, count, [](const segmi_muon_matrix& a) { return shape_of(a.rows, a.cols, true); }); }
 
 }  // namespace
 
@@ -1671,7 +1894,7 @@ size_t segmi_ns_workspace(const segmi_ns_matrix* mats_host, int count) {
     if (!mats_host || count <= 0) return 0;
     for (int i = 0; i < count; ++i)
         if (!shape_ok(mats_host[i].rows, mats_host[i].cols)) return 0;
-    return workspace_of(mats_host, count, [](const segmi_ns_matrix& a) { return shape_of(a); });
+    return need_of(mats_host, count).bytes();
 }
 
 int segmi_ns_coefficients_ok(const double* coefficients_host, int steps) {
@@ -1687,11 +1910,14 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
         if (!a.src || !a.dst || !shape_ok(a.rows, a.cols) || a.dtype < 0 || a.dtype > 1) return SEGMI_ERR_BADARG;
     }
     if ((size_t)workspace & 255) return SEGMI_ERR_ALIGN;
-    if (workspace_bytes < segmi_ns_workspace(mats_host, count)) return SEGMI_ERR_WORKSPACE;
+    const Need need = need_of(mats_host, count);
+    if (!need.bytes() || workspace_bytes < need.bytes()) return SEGMI_ERR_WORKSPACE;
+    char* const thin = static_cast<char*>(workspace);
+    char* const rest = thin + need.thin;
     const Bounds f{coefficients_host[0], coefficients_host[1], coefficients_host[2]};
     Aside aside((hipStream_t)stream, mixed(mats_host, count));
     return aside.join(for_batches(mats_host, count, [&](Class cls, const int* index, int k) {
-        if (cls < SQUARE) {
+        if (cls < THIN) {
             SmallBatch b{};
             b.eps = eps;
             for (int i = 0; i < k; ++i) {
@@ -1727,7 +1953,8 @@ int segmi_ns_orthogonalize(const segmi_ns_matrix* mats_host, int count, const do
             t.dtype = a.dtype;
             t.turned = t.si == 1 && t.sj != 1;
         }
-        return run_batch<false>(cls == WIDE_MATRIX, shapes, src, dst, k, f, steps, static_cast<char*>(workspace), Hyper{}, nullptr, (hipStream_t)stream);
+        if (cls == THIN) return run_thin<false>(shapes, src, dst, k, f, steps, thin, Hyper{}, nullptr, aside.stream());
+        return run_batch<false>(cls == WIDE_MATRIX, shapes, src, dst, k, f, steps, rest, Hyper{}, nullptr, (hipStream_t)stream);
     }));
 }
 
@@ -1735,7 +1962,7 @@ size_t segmi_muon_workspace(const segmi_muon_matrix* mats_host, int count) {
     if (!mats_host || count <= 0) return 0;
     for (int i = 0; i < count; ++i)
         if (!shape_ok(mats_host[i].rows, mats_host[i].cols)) return 0;
-    return workspace_of(mats_host, count, [](const segmi_muon_matrix& a) { return shape_of(a.rows, a.cols, true); });
+    return need_of(mats_host, count).bytes();
 }
 
 int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* lr_host, const float* weight_decay_host,
@@ -1749,7 +1976,10 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
         if (!a.param || !a.grad || !a.momentum || !shape_ok(a.rows, a.cols) || a.group < 0 || a.group >= ngroups) return SEGMI_ERR_BADARG;
     }
     if ((size_t)workspace & 255) return SEGMI_ERR_ALIGN;
-    if (workspace_bytes < segmi_muon_workspace(mats_host, count)) return SEGMI_ERR_WORKSPACE;
+    const Need need = need_of(mats_host, count);
+    if (!need.bytes() || workspace_bytes < need.bytes()) return SEGMI_ERR_WORKSPACE;
+    char* const thin = static_cast<char*>(workspace);
+    char* const rest = thin + need.thin;
     const Bounds f{coefficients_host[0], coefficients_host[1], coefficients_host[2]};
     Hyper h{};
     if (!hyper_dev)
@@ -1760,7 +1990,7 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
         }
     Aside aside((hipStream_t)stream, mixed(mats_host, count));
     return aside.join(for_batches(mats_host, count, [&](Class cls, const int* index, int k) {
-        if (cls < SQUARE) {
+        if (cls < THIN) {
             SmallBatch b{};
             b.eps = eps;
             b.nesterov = nesterov;
@@ -1801,8 +2031,9 @@ int segmi_muon_step(const segmi_muon_matrix* mats_host, int count, const float* 
             t.group = a.group;
             t.turned = !wide;
         }
-        return run_batch<true>(cls == WIDE_MATRIX, shapes, src, dst, k, f, steps, static_cast<char*>(workspace), h, reinterpret_cast<const Hyper*>(hyper_dev),
-                               (hipStream_t)stream);
+        if (cls == THIN)
+            return run_thin<true>(shapes, src, dst, k, f, steps, thin, h, reinterpret_cast<const Hyper*>(hyper_dev), aside.stream());
+        return run_batch<true>(cls == WIDE_MATRIX, shapes, src, dst, k, f, steps, rest, h, reinterpret_cast<const Hyper*>(hyper_dev), (hipStream_t)stream);
     }));
 }
 
