@@ -511,8 +511,9 @@ int segmi_sgd_step_dev(const segmi_sgd_chunk* table, int nchunks, const float* h
  *
  * Orthogonalisation by Newton-Schulz products: X = G / max(|G|_F, eps), then `steps` times
  *     X <- (a I + b X X^T + c (X X^T)^2) X        (on the shorter side of G; a, b, c = coefficients_host[0..2])
- * dst = X in G's type.  Element (r, c) of a matrix lies at r * rs + c * cs (elements; any strides, also 0 in src).  fp32 accuracy
- * (products of fp16 pairs, fp32 accumulators); NaN or infinity anywhere in a matrix makes all of its result NaN.  `dst` must not
+ * dst = X in G's type.  Element (r, c) of a matrix lies at r * rs + c * cs (elements; any strides, also 0 in src).  The accuracy
+ * of an fp32 iteration over a matrix (products of fp16 pairs, fp32 accumulators); beside it a value is off by up to 2^-39 of the matrix's
+ * norm, which shows in rows or columns below 1e-4 of that norm (1e-6: up to 3e-4 of the row).  NaN or infinity anywhere in a matrix makes all of its result NaN.  `dst` must not
  * overlap any `src`.  The descriptor arrays are HOST memory, read before the call returns; the workspace is aligned to 256 bytes. */
 #define SEGMI_NS_MAX_STEPS 32
 typedef struct segmi_ns_matrix {

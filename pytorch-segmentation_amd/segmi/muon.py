@@ -72,7 +72,8 @@ def orthogonalize(matrices, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
 
     `matrices`: a float32 or bfloat16 CUDA tensor of two or more dimensions (seen as shape[0] x the rest), or a list of them, any sizes
     and strides; all of them share the launches.  Returns new tensors of the same shapes, types and (where dense) strides.  Computed
-    to fp32 accuracy in both types; the last bits may depend on what else is in the list.  No gradient is recorded.  A matrix that holds NaN or infinity comes back as NaN, a zero one as zero.
+    in both types to the accuracy of an fp32 iteration over a matrix.  Values are held to 2^-22 of themselves and 2^-39 of the matrix's norm: a row or
+    column that is 1e-6 of the matrix comes out to 4e-5 (64 x 576) - 3e-4 (300 x 5000) of its own size, in fp32 to 1e-5.  The last bits may depend on what else is in the list.  No gradient is recorded.  A matrix that holds NaN or infinity comes back as NaN, a zero one as zero.
     Runs on the current stream of the tensors' device; may be captured into a hipGraph."""
     single = isinstance(matrices, torch.Tensor)
     mats = [matrices] if single else list(matrices)
