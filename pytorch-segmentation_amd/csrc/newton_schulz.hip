@@ -19,8 +19,8 @@
 // of the fp16 rate = 5 times the fp32 matrix rate.  fp16's range is no obstacle here: the iterates' singular values are bounded by
 // intervals that follow from the coefficients (`Bounds` below), so each matrix gets the scale that puts its bound below 2^15; what is
 // lost below fp16's subnormal step is at most 2^-25 / 2^14 = 2^-39 of the largest possible entry.  fp32 would keep the relative accuracy of small
-values: rows (or columns) from 1 down to 1e-4 come out as in fp32, in 1e-6 the worst row is off by 4e-5 (64 x 576), 1.1e-4 (256 x 1024), 2.5e-4 (300 x
-5000), fp32's by 3e-6 - 1e-5, in 1e-8 by 4e-3, 9e-3, 2e-2.
+// values: rows (or columns) from 1 down to 1e-4 come out as in fp32, in 1e-6 the worst row is off by 4e-5 (64 x 576), 1.1e-4 (256 x 1024), 2.5e-4 (300 x
+// 5000), fp32's by 3e-6 - 1e-5, in 1e-8 by 4e-3, 9e-3, 2e-2.
 //
 // Symmetric products compute the tiles on and below the diagonal and store each twice.
 //
