@@ -1,16 +1,17 @@
 // Fused AdamW step (decoupled weight decay) over a set of tensors.
 //     m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = (1 - lr wd) p - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // HBM-bound: 28 B per parameter (read p, g, m, v; write p, m, v): all of PSPNet-R50's, 1.44 GB, in 283 us = 5.1 TB/s, above what a copy reaches
-// (4.7).  Up to 56 tensors travel as kernel arguments, so nothing is
-// uploaded and gradients may move from step to step at no cost; a workgroup finds its tensor with one load and a ballot over the
-// tensors' first workgroups.
+// (4.7).  Up to 56 tensors travel as kernel arguments, so nothing is uploaded when gradients move from step to step (the host makes
+// their descriptors anew: 0.88 instead of 0.13 ms of its time for those 187 tensors); a workgroup finds its tensor with one load and a ballot
+// over the tensors' first workgroups.
 #include "segmi_common.h"
 #include <cmath>
 
 namespace {
 
 constexpr int MAX_GROUPS = 8;
-constexpr int BATCH = 56;            // 64 B a tensor: with the hyper-parameters below the 4 KiB of kernel arguments
+constexpr int BATCH = 56;            // 56 B a tensor: with the hyper-parameters below the 4 KiB of kernel arguments
+static_assert(BATCH <= 64, "a lane looks at a tensor");
 constexpr int CHUNK = 4096;          // elements per workgroup: four 16-byte vectors per thread and stream
 
 struct AdamTensor {
@@ -33,6 +34,7 @@ struct AdamBatch {
     AdamTensor t[BATCH];
     AdamHyper h[MAX_GROUPS];
 };
+static_assert(sizeof(AdamTensor) == 56 && sizeof(AdamBatch) + 2 * sizeof(void*) < 4096, "kernel arguments");
 
 __device__ __forceinline__ float adam_one(float p, float g, float& m, float& v, const AdamHyper& h, float lr1, float rbc2) {
     m = fmaf(h.b1, m, h.c1 * g);

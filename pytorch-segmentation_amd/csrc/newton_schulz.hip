@@ -45,7 +45,8 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int BATCH = 60;            // matrices per launch: their descriptors travel as kernel arguments (< 4 KiB)
+constexpr int BATCH = 60;            // matrices per launch: their descriptors travel as kernel arguments (< 4 KiB, asserted at each)
+static_assert(BATCH <= 64, "a lane looks at a matrix");
 constexpr int MAX_GROUPS = 8;
 constexpr unsigned LINE = 64, LINE_K = 16;   // bytes, values
 
@@ -144,6 +145,10 @@ struct SourceBatch {
 struct Hyper {
     float lr[MAX_GROUPS], wd[MAX_GROUPS], mom[MAX_GROUPS];
 };
+// descriptors, by-value hyper-parameters and the pointer to those on the device, with eight bytes of padding
+template <typename B>
+constexpr bool fits_arguments = sizeof(B) + sizeof(Hyper) + 2 * sizeof(void*) < 4096;
+static_assert(fits_arguments<SourceBatch>, "kernel arguments");
 
 __device__ __forceinline__ float bf16_to_f32(unsigned short u) { return __uint_as_float((unsigned)u << 16); }
 __device__ __forceinline__ unsigned short f32_to_bf16(float f) {
@@ -567,6 +572,7 @@ struct Product {
     float scale;                     // fp32 sum -> stored result
     float ident, lin;                // out = ident I + lin A + scale L R^T (POLY only; A in its stored scale)
 };
+static_assert(sizeof(Batch) + sizeof(Product) < 4096, "kernel arguments");
 
 // m x m products (all operands symmetric): A^2 with the polynomial's epilogue, Q A, W Q, P Q.
 template <typename C, bool POLY>
@@ -616,6 +622,7 @@ struct GramBatch {
     float scale;
     GramItem item[BATCH];
 };
+static_assert(sizeof(GramBatch) < 4096, "kernel arguments");
 
 template <typename C>
 __global__ __launch_bounds__(256, C::PER_CU) void ns_gram(GramBatch b) {
@@ -741,6 +748,7 @@ struct TargetBatch {
     float scale, alpha;              // of the stored sum, of the stored X (as in ns_apply)
     Target item[BATCH];
 };
+static_assert(fits_arguments<TargetBatch>, "kernel arguments");
 
 // MUON: param = param (1 - lr wd) - lr factor O, else dst = O
 template <typename C, bool MUON>
@@ -836,6 +844,7 @@ struct SmallBatch {
     SmallStep step[SEGMI_NS_MAX_STEPS];
     SmallItem item[SMALL_BATCH];
 };
+static_assert(fits_arguments<SmallBatch>, "kernel arguments");
 
 // two values' pairs: hi of both in one register, lo of both in another; the mixed-precision instructions take the halves as they lie
 struct Pair2 {
@@ -1261,7 +1270,7 @@ struct ThinBatch {
     int count, nesterov;
     ThinItem item[THIN_BATCH];
 };
-static_assert(sizeof(ThinBatch) + sizeof(Hyper) + 2 * sizeof(void*) < 4096, "kernel arguments");
+static_assert(THIN_BATCH <= BATCH && fits_arguments<ThinBatch>, "kernel arguments");
 constexpr int THIN_TILE = 256;       // columns at a time
 // Columns per workgroup: at most 256 workgroups a matrix, so that adding their parts stays short.
 __host__ __device__ inline unsigned thin_columns(int n) { return THIN_TILE * (((unsigned)n + 256u * THIN_TILE - 1) / (256u * THIN_TILE)); }
