@@ -7,7 +7,8 @@
 
 All three are reached through `segmi.optim`, and the two optimizers by name from config.json (`"optimizer": {"type": "Muon", ...}`), the
 way the reference resolves its optimizers (`base/base_trainer.py:57`).  `AdamW` in a config stays torch.optim.AdamW.
-Pointers travel as kernel arguments: no table is uploaded, gradients may move between steps, nothing waits for the GPU.
+Pointers travel as kernel arguments: no table is uploaded, gradients may move between steps (the host then makes the descriptors anew), nothing
+waits for the GPU.
 """
 import contextlib
 import ctypes as C
@@ -259,7 +260,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
     def _checked(self, p):
         g = p.grad
         if not (p.is_cuda and p.dtype == torch.float32 and not g.is_sparse and g.dtype == torch.float32 and g.device == p.device and
-                _same_layout(g, p) and _unit_of(p.shape, p.stride()) == 1):
+                (g.shape == p.shape and g.stride() == p.stride() or _same_layout(g, p)) and (p.is_contiguous() or _unit_of(p.shape, p.stride()) == 1)):
             raise RuntimeError("%s: parameters and gradients must be float32 CUDA tensors on one device with identical (dense) strides" % self._name())
         if p.is_neg() or g.is_neg():
             raise RuntimeError("%s: a parameter or gradient is a negated view; resolve_neg() makes one the kernels can read" % self._name())

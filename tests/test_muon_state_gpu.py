@@ -70,3 +70,16 @@ def test_negated_views_are_what_they_stand_for(cuda):
     for cls in (optim.Muon, optim.FusedAdamW):
         with pytest.raises(RuntimeError, match="negated"):
             cls([p]).step()
+
+
+@pytest.mark.parametrize("cls", ["Muon", "FusedAdamW"])
+def test_gradients_of_another_shape_are_refused(cuda, cls):
+    """`p.data = ...` lets a parameter outgrow its gradient."""
+    for shape, larger in (((8,), (16,)), ((6, 5), (12, 5))):
+        p = torch.nn.Parameter(torch.zeros(shape, device=cuda))
+        p.grad = torch.ones(shape, device=cuda)
+        opt = getattr(optim, cls)([p])
+        opt.step()
+        p.data = torch.zeros(larger, device=cuda)
+        with pytest.raises(RuntimeError):
+            opt.step()
