@@ -23,11 +23,8 @@ ARCH = "gfx950"
 # no packed fp32 arithmetic (v_pk_add/mul/fma_f32) in any kernel: some of its forms have given wrong results on this hardware now and then
 FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Wno-unused-value",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# per-file additions: no compiler-formed packed-fp32 arithmetic (v_pk_mul/fma/add_f32) in the HBM-bound kernels.  The SLP-packed
-# form of bilinear_fwd_kernel returns wrong high halves while a bf16x3 convolution kernel of ANOTHER process shares the GPU
-# (tools/probes/pk_two_process.py reproduces it with exactly these two kernels: 32 % of the launches wrong against an fp64 reference,
-# profiles/r03_pk_two_process_ref.txt);
-# the scalar form never does.  These kernels are HBM-bound: no cost.
+# per-file additions: the HBM-bound kernels are built without the vectorisers, which formed that arithmetic there before FLAGS ruled it out
+# (bilinear_fwd_kernel then gave wrong high halves beside another process's matrix kernels); their instruction order was tuned this way
 EXTRA_FLAGS = {f: ["-fno-slp-vectorize", "-fno-vectorize"] for f in ("pool_resize.hip", "conv_winograd.hip", "bn.hip", "loss.hip", "misc.hip", "optim.hip",
                                                     "lovasz.hip", "dwconv_shuffle.hip", "pyramid_bottleneck.hip", "augment.hip")}
 
@@ -51,7 +48,7 @@ def _stale(target, deps):
 
 def build(force=False, verbose=True):
     os.makedirs(OBJ_DIR, exist_ok=True)
-    srcs, hdrs = _sources(), _headers()
+    srcs, hdrs = _sources(), _headers() + [os.path.abspath(__file__)]      # (another set of flags is another object)
     jobs = []
     for s in srcs:
         o = os.path.join(OBJ_DIR, os.path.basename(s)[:-4] + ".o")
