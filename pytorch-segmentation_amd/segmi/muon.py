@@ -293,7 +293,7 @@ class _FusedOptimizer(torch.optim.Optimizer):
         if (k is not None and len(flat) == len(k["flat"]) and all(map(is_, flat, k["flat"])) and missing == k["missing"] and
                 list(map(_ptr, live)) == k["grad_ptrs"] and self._strides(flat, live, k["deep"], k["shallow"]) == k["strides"]):
             held = list(chain.from_iterable(map(dict.values, k["states"])))
-            if (all(map(is_, map(self.state.get, k["owners"]), k["states"])) and
+            if (len(self.state) == len(k["owners"]) and all(map(is_, self.state.values(), k["dicts"])) and all(map(is_, self.state, k["owners"])) and
                     len(held) == len(k["held"]) and all(map(is_, held, k["held"])) and list(map(_ptr, k["tensors"])) == k["ptrs"] and
                     list(map(_numel, flat)) == k["numels"] and [p.shape for _, p in k["members"]] == k["shapes"] and
                     list(map(len, map(_params, self.param_groups))) == k["lengths"] and self._settings() == k["settings"]):
@@ -316,14 +316,13 @@ class _FusedOptimizer(torch.optim.Optimizer):
             k["rest"] = self._adamw_descriptors(rest)
             k["rows"] = None if self.capturable else np.array([self._step_of[p] for _, p in rest])
         self._check_apart(k["mats"][0] if mats else None, k["rest"])
-        owners = [p for _, p in mats + rest]
-        states = [self.state[p] for p in owners]
+        states = [self.state[p] for _, p in mats + rest]
         held = list(chain.from_iterable(map(dict.values, states)))
         tensors = flat + [t for st in states for key, t in st.items() if (key != "step" or self.capturable) and isinstance(t, torch.Tensor)]
         deep = [(i, j) for j, i in enumerate(i for i, g in enumerate(grads) if g is not None) if grads[i].dim() > 1]      # (among the parameters, among the gradients)
         shallow = [j for j, g in enumerate(live) if g.dim() == 1]
         k.update(flat=flat, missing=missing, grad_ptrs=list(map(_ptr, live)), deep=deep, shallow=shallow,
-                 strides=self._strides(flat, live, deep, shallow), owners=owners, states=states, held=held,
+                 strides=self._strides(flat, live, deep, shallow), owners=list(self.state), dicts=list(self.state.values()), states=states, held=held,
                  tensors=tensors, ptrs=list(map(_ptr, tensors)), numels=list(map(_numel, flat)), members=mats, shapes=[p.shape for _, p in mats],
                  lengths=list(map(len, map(_params, self.param_groups))), settings=self._settings())
         self._kept = k

@@ -354,3 +354,20 @@ def test_a_load_without_state_and_without_a_graph_leaves_none(host, cls):
     assert not opt.state_dict()["state"]
     opt.step()
     assert all(float(st["step"]) == 1.0 for st in opt.state.values() if "step" in st)
+
+
+@pytest.mark.parametrize("cls", OPTIMIZERS)
+def test_state_dictionaries_that_change_places_are_seen(host, cls):
+    a, b = (torch.nn.Parameter(torch.zeros(80, 70)) for _ in range(2))
+    for p in (a, b):
+        p.grad = torch.ones_like(p)
+    opt = cls([a, b])
+    opt.step()
+    key = next(k for k in opt.state[a] if k != "step")
+    opt.state[a], opt.state[b] = opt.state[b], opt.state[a]
+    opt.step()
+    name, field = ("muon", "momentum") if cls is optim.Muon else ("adamw", key)
+    assert {int(r["param"]): int(r[field]) for r in host.last(name)} == {p.data_ptr(): opt.state[p][key].data_ptr() for p in (a, b)}
+    opt.state[torch.nn.Parameter(torch.zeros(3))] = {}        # another's: nothing changes here
+    opt.step()
+    assert {int(r["param"]): int(r[field]) for r in host.last(name)} == {p.data_ptr(): opt.state[p][key].data_ptr() for p in (a, b)}
