@@ -1247,8 +1247,8 @@ __global__ __launch_bounds__(512, 2) void ns_small(SmallBatch b, Hyper h, const 
 // Distance from 64-bit results (root mean square of 16 matrices): 16 x 4608 6e-8, noise with strong directions 1.6e-7; as fp16 pairs through the
 // products above 1.3e-6, the fp32 iteration 1.0e-6.  Time, here / there: 3 x 5000 57 / 94 us, 16 x 36864 113 / 152, 16 x 10^6 656 / 1046, 32 of
 // 8 x 10000 168 / 358; 16 x 4608 beside 256 x 1024, which it no longer shares launches with, 188 / 134, beside a network's filters nothing.
-// Bound by latency up to some 10^5 columns (seven launches), then by LDS, which serves two fp32 operands of every 64-bit product (16 x 16 000 000:
-// 8.6 ms for 12 GB of X, 1.4 TB/s).
+// Bound by latency: seven launches, of 9 us each for 3 x 5000 and 19 for 16 x 36864, and from some 10^5 columns on that of the 64-bit products of four
+// waves a CU, whose operands come from LDS (16 x 16 000 000: 1.4 ms a step for 2 GB of X, 1.5 TB/s; without the Gram matrix no less).
 struct ThinItem {
     const void* src;                 // MUON: the gradient
     void* dst;                       // MUON: the parameter
