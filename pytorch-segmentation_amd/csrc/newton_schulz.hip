@@ -1460,7 +1460,11 @@ Class class_of(int rows, int cols, size_t span) {
     return is_wide(m, n) ? WIDE_MATRIX : SQUARE;
 }
 size_t span_of(const segmi_ns_matrix& a) {
-    const auto end = [&](long rs, long cs) { return ((size_t)(a.rows - 1) * rs + (size_t)(a.cols - 1) * cs + 1) * (a.dtype ? 2 : 4); };
+    constexpr size_t FAR = (size_t)1 << 62;              // a negative stride, or no sum of 64 bits: not for 32-bit offsets
+    const auto end = [&](long rs, long cs) {
+        if (rs < 0 || cs < 0 || (double)(a.rows - 1) * (double)rs + (double)(a.cols - 1) * (double)cs > 1e15) return FAR;
+        return ((size_t)(a.rows - 1) * rs + (size_t)(a.cols - 1) * cs + 1) * (a.dtype ? 2 : 4);
+    };
     return std::max(end(a.src_rs, a.src_cs), end(a.dst_rs, a.dst_cs));
 }
 size_t span_of(const segmi_muon_matrix& a) { return (size_t)a.rows * a.cols * 4; }
