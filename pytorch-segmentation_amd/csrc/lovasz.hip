@@ -145,6 +145,17 @@ struct LovRow {
 // trips of lane g over its groups (KQ > 0: compile-time, groups past the row are zeros and every use is guarded by c < C)
 #define LOV_TRIPS(KQ, g, c4n) (KQ > 0 ? KQ : ((c4n) - (g) + 7) / 8)
 
+// Kernels, not hipMemsetAsync: a captured graph's memset nodes have given wrong values on this hardware from the second replay on.
+__global__ __launch_bounds__(256) void lovasz_clear_kernel(unsigned* __restrict__ counts, unsigned* __restrict__ thr, int C) {
+    for (int i = threadIdx.x; i <= C; i += 256) {
+        counts[i] = 0u;
+        if (i < C) thr[i] = 0xFFFFFFFFu;
+    }
+}
+__global__ __launch_bounds__(256) void lovasz_zero_kernel(unsigned* __restrict__ p, long n) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) p[i] = 0u;
+}
+
 // 8 lanes share a pixel (float4 channel groups, xor-shuffle reductions): coalesced 128-byte row segments
 template <int KQ, bool UP>
 __global__ __launch_bounds__(256) void lovasz_prepare_kernel(const LovSrc src, const int64_t* __restrict__ target,
@@ -993,8 +1004,7 @@ int lovasz_fwd_impl(const LovSrc lsrc, bool up, const int64_t* target, long rows
     double* part = (double*)(ws + L.part);
     const int prune = lovasz_prune() ? 1 : 0;
 
-    hipMemsetAsync(counts, 0, (size_t)(C + 1) * 4, st);
-    hipMemsetAsync(thr, 0xFF, (size_t)C * 4, st);
+    hipLaunchKernelGGL(lovasz_clear_kernel, dim3(1), dim3(256), 0, st, counts, thr, C);
     long pb = (rows + 31) / 32;
     if (pb > SEGMI_MAX_GRID) pb = SEGMI_MAX_GRID;
     const int kq = lov_kq(C);
@@ -1033,7 +1043,10 @@ int lovasz_fwd_impl(const LovSrc lsrc, bool up, const int64_t* target, long rows
         hipLaunchKernelGGL(segsort_hist_kernel, tgrid, dim3(256), 0, st, (const unsigned long long*)src, rows, L.ntiles, shift, mask, (const unsigned*)nkept, hist);
         hipLaunchKernelGGL(segsort_scan_kernel, dim3((unsigned)C), dim3(256, SCAN_Q), 0, st, hist, L.ntiles, (const unsigned*)nkept);
         const bool count_fg = pass == 3 && fused_fg;
-        if (count_fg) hipMemsetAsync(chunk_fg, 0, (size_t)C * L.nchunks * sizeof(unsigned), st);
+        if (count_fg) {
+            const long words = (long)C * L.nchunks, zgrid = (words + 255) / 256;
+            hipLaunchKernelGGL(lovasz_zero_kernel, dim3((unsigned)(zgrid < 1024 ? zgrid : 1024)), dim3(256), 0, st, chunk_fg, words);
+        }
         hipLaunchKernelGGL(segsort_scatter_kernel, tgrid, dim3(256), 0, st, (const unsigned long long*)src, dst, rows, L.ntiles, shift, mask,
                            (const unsigned*)nkept, (const unsigned*)hist, count_fg ? chunk_fg : (unsigned*)nullptr, L.nchunks, L.PB);
         unsigned long long* t = src; src = dst; dst = t;
